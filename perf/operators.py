@@ -146,7 +146,7 @@ def _exponent(amax, kind):
 
 def _power(e):
     """2**e as fp32, NaN for the exponent that marks a block without a scale."""
-    return torch.where(e == 128, math.nan, torch.ldexp(torch.ones((), device=e.device), e.clamp(max=127)))
+    return torch.where(e == 128, math.nan, torch.ldexp(torch.ones_like(e, dtype=torch.float32), e.clamp(max=127)))
 
 
 def _round(x, kind):
