@@ -128,6 +128,21 @@ void dp_muon_prepare(torch::Tensor grad_ptrs, int64_t rank, int64_t world, torch
                      double extra_sq, double max_norm);
 void dp_muon_apply_allgather(torch::Tensor param_ptrs, int64_t rank, int64_t world, torch::Tensor offs,
                              int64_t numel, double decay, double step_scale, torch::Tensor orth);
+// kv8_cache.cu, kv8_attention.cu (8-bit key/value cache)
+void kv8_append(torch::Tensor keys, torch::Tensor values, torch::Tensor key_scales, torch::Tensor value_scales,
+                int64_t block, torch::Tensor k, torch::Tensor v, torch::Tensor seqlens);
+std::vector<torch::Tensor> kv8_read(torch::Tensor keys, torch::Tensor values, torch::Tensor key_scales,
+                                    torch::Tensor value_scales, int64_t block, torch::Tensor seqlens,
+                                    c10::optional<torch::Tensor> start, int64_t start0, int64_t length);
+torch::Tensor kv8_attend(torch::Tensor q, torch::Tensor keys, torch::Tensor values, torch::Tensor key_scales,
+                         torch::Tensor value_scales, int64_t block, c10::optional<torch::Tensor> k,
+                         c10::optional<torch::Tensor> v, torch::Tensor seqlens, double scale, int64_t left,
+                         int64_t right);
+// logprobs.cu
+std::vector<torch::Tensor> logprobs_fwd(torch::Tensor logits, torch::Tensor tokens, int64_t top, int64_t ignore);
+torch::Tensor logprobs_bwd(torch::Tensor logits, torch::Tensor tokens, int64_t ignore, torch::Tensor lse,
+                           torch::Tensor entropy, torch::Tensor top_tok, c10::optional<torch::Tensor> g_lp,
+                           c10::optional<torch::Tensor> g_ent, c10::optional<torch::Tensor> g_top);
 }  // namespace mykb
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -183,6 +198,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fp8_scaled_gemm", &mykb::fp8_scaled_gemm, "per-tensor / per-row scaled float8 GEMM on tcgen05");
   m.def("fa_decode", &mykb::fa_decode);
   m.def("kv_append", &mykb::kv_append);
+  m.def("kv8_append", &mykb::kv8_append, "quantise new keys / values into an 8-bit cache");
+  m.def("kv8_read", &mykb::kv8_read, "bf16 copies of a range of an 8-bit cache");
+  m.def("kv8_attend", &mykb::kv8_attend, "append to an 8-bit cache and attend over it");
+  m.def("logprobs_fwd", &mykb::logprobs_fwd, "token log-probs, entropy and top alternatives of logits");
+  m.def("logprobs_bwd", &mykb::logprobs_bwd);
   m.def("ngram_adam", &mykb::ngram_adam);
   m.def("peer_barrier", &mykb::peer_barrier);
   m.def("dp_reduce_sumsq", &mykb::dp_reduce_sumsq);

@@ -1,0 +1,599 @@
+// Attention over the 8-bit key/value cache (formats and scales: kv8.cuh).
+//
+//   o_r = sum_j p_rj v_j,  p = softmax_j(scale q_r.k_j),  k_j = s_kj kq_j,  v_j = s_vj vq_j
+//
+// with the scales taken out of the products: t_rj = scale log2(e) s_kj (q_r.kq_j) + log2 s_vj,
+// w_rj = 2^(t_rj - m_r), o_r = sum w vq / sum w 2^(-log2 s_vj), where m_r follows the row's
+// maximum of t.  Both products run on the tensor cores (f16 x f16 -> fp32): e4m3 and int8
+// values are exact in f16; a query row is multiplied by a power of two that brings its largest
+// element just under 2^15 (bf16's 8 bits are exact in f16 there; elements below 2^-29 of the
+// largest fade out); w is rounded to f16's 11 bits, and m_r is kept such that the largest w
+// lies in 2^8 .. 2^15, so weights down to 2^-32 of the largest survive the rounding and O is
+// rescaled only when a row's maximum grows by more than 2^7.  Sums, maxima and O are fp32.
+//
+// A decode step reads every visible byte of the cache once and does little with it, so it is
+// bound by HBM.  One work list holds the 16-key-multiple tiles of all (sequence, KV head,
+// 16-row tile) columns; every CTA takes an equal run of it, computed on the device from the
+// lengths (ragged batches stay balanced, a captured CUDA graph stays valid).  The four warps
+// of a CTA take its tiles in turn; each lane copies exactly the bytes that it will feed to the
+// MMAs into its own slots of shared memory (cp.async, several tiles ahead), so there are no
+// bank conflicts, barriers or transposes: the contraction index of Q K^T and the column index
+// of P V are permuted to make a lane's bytes contiguous in memory.
+// A column that one CTA covers is written at once; else the CTAs leave fp32 partials and the
+// last one to finish (a ticket; nothing waits) joins them in order, so results do not depend
+// on timing.
+#include <torch/extension.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include "kv8.cuh"
+#include "kv8_host.h"
+
+namespace mykb {
+std::vector<torch::Tensor> fa_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, c10::optional<torch::Tensor> cu_q,
+                                  c10::optional<torch::Tensor> cu_k, c10::optional<torch::Tensor> seqused_k,
+                                  int64_t max_q, int64_t max_k, double scale, int64_t left, int64_t right);
+namespace kv8 {
+
+constexpr int ROWS = 16;   // query rows of one MMA tile
+constexpr int WARPS = 4;
+constexpr int THREADS = WARPS * 32;
+
+struct AttendParams {
+  const bf16* q;       // (B, L, H, D)
+  const uint8_t* k;    // (B, Hkv, cap, D)
+  const uint8_t* v;
+  const uint8_t* ks;   // (B, Hkv, nblk)
+  const uint8_t* vs;
+  const int* seqlens;  // (B)
+  bf16* o;             // (B, L, H, D) contiguous
+  float* part;         // [grid][2][rows <= 16][D] partial O, columns permuted (see flush)
+  float* ml;           // [grid][2][16][2]
+  int* tickets;        // [B * Hkv * RT], zero
+  int64_t q_sb, q_st, q_sh;
+  int B, L, H, Hkv, RT, cap, nblk, shift;
+  int extra;           // visible keys = seqlens + extra
+  int left, right;
+  float scale_log2;    // |softmax scale| * log2(e)
+  float sign;
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// Shape of the kernel for one head_dim: keys a tile, tiles in the ring, CTAs an SM.
+template <int D>
+struct Shape {
+  static constexpr int KT = 32;
+  static constexpr int STAGES = 3;
+  static constexpr int TILE = KT * D * 2;  // bytes of a tile's keys and values
+  static constexpr int RING = WARPS * STAGES * TILE;
+  static constexpr int OROW = D + 8;       // floats of a row in the merge buffer: conflict-free float2 writes
+  static constexpr int SMEM = RING > WARPS * ROWS * OROW * 4 ? RING : WARPS * ROWS * OROW * 4;
+  static constexpr int PER_SM = D == 64 ? 3 : 2;
+};
+
+// Tiles of a sequence that some query sees: [t0, t0 + n).
+template <int KT>
+__device__ __forceinline__ int2 tiles_of(const AttendParams& p, int b, int& kv_len) {
+  kv_len = (int)min((int64_t)max(p.seqlens[b], 0) + p.extra, (int64_t)p.cap);
+  if (kv_len <= 0) return make_int2(0, 0);
+  const int lo = p.left >= 0 ? (int)max((int64_t)0, (int64_t)kv_len - p.L - p.left) : 0;
+  const int t0 = lo / KT;
+  return make_int2(t0, (kv_len + KT - 1) / KT - t0);
+}
+
+// UNI: a scale block spans whole 16-key groups (block >= 16), else each key has its own lookup.
+template <int D, bool INT8, bool UNI>
+__global__ void __launch_bounds__(THREADS, Shape<D>::PER_SM) attend_kernel(AttendParams p) {
+  using S = Shape<D>;
+  constexpr int KT = S::KT, STAGES = S::STAGES, U = KT / 16, HALVES = D / 64, VB = D / 8;
+  extern __shared__ __align__(128) unsigned char ring[];
+  __shared__ int64_t scan[THREADS + 1];
+  __shared__ int64_t start_base;
+  __shared__ int start_b, last;
+  __shared__ float wM[WARPS][ROWS], wL[WARPS][ROWS], rM[ROWS], rL[ROWS];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  const int G = p.H / p.Hkv, rows_all = G * p.L;
+  const int cols = p.Hkv * p.RT;  // columns a sequence
+
+  // ---- the work list: each thread sums a run of sequences, then a scan over the threads
+  const int run = (p.B + THREADS - 1) / THREADS;
+  int64_t mine = 0;
+  for (int i = 0; i < run; ++i) {
+    const int b = tid * run + i;
+    int kl;
+    if (b < p.B) mine += tiles_of<KT>(p, b, kl).y;
+  }
+  {
+    int64_t x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    __shared__ int64_t wsum[WARPS];
+    if (lane == 31) wsum[warp] = x;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) x += wsum[w];
+    scan[tid + 1] = x;
+    if (tid == 0) scan[0] = 0;
+    __syncthreads();
+  }
+  const int64_t total = scan[THREADS] * cols;
+  // as many CTAs take part as get at least one tile a warp
+  const int64_t active = min((int64_t)gridDim.x, (total + WARPS - 1) / WARPS);
+  // sequences without visible keys: their rows are 0
+  for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
+    int kl;
+    if (tiles_of<KT>(p, b, kl).y > 0) continue;
+    uint32_t* o = reinterpret_cast<uint32_t*>(p.o + (int64_t)b * p.L * p.H * D);
+    for (int64_t i = tid; i < (int64_t)p.L * p.H * D / 2; i += THREADS) o[i] = 0;
+  }
+  if (blockIdx.x >= active) return;
+  auto first_of = [&](int64_t cta) { return total * cta / active; };
+  int64_t pos = first_of(blockIdx.x);
+  const int64_t end = first_of(blockIdx.x + 1);
+  if (scan[tid] * cols <= pos && pos < scan[tid + 1] * cols) {
+    int64_t base = scan[tid] * cols;
+    int b = tid * run;
+    for (;; ++b) {
+      int kl;
+      const int64_t n = (int64_t)tiles_of<KT>(p, b, kl).y * cols;
+      if (pos < base + n) break;
+      base += n;
+    }
+    start_b = b, start_base = base;
+  }
+  __syncthreads();
+  int b = start_b;
+  int64_t base = start_base;
+  const uint32_t slot0 = smem_u32(ring) + warp * (STAGES * S::TILE);
+  const float ninf = -INFINITY;
+
+  while (pos < end) {
+    int kv_len;
+    const int2 tl = tiles_of<KT>(p, b, kv_len);
+    const int nt = tl.y;
+    if (pos >= base + (int64_t)nt * cols) {
+      base += (int64_t)nt * cols;
+      ++b;
+      continue;
+    }
+    const int col = (int)((pos - base) / nt);
+    const int ta = (int)((pos - base) - (int64_t)col * nt);          // first tile of this piece
+    const int n = (int)min((int64_t)(nt - ta), end - pos);            // its tiles
+    const int hk = col / p.RT, rt = col % p.RT;
+    const int rows = min(ROWS, rows_all - rt * ROWS);
+    const int64_t bh = (int64_t)b * p.Hkv + hk;
+    const uint8_t* kb = p.k + bh * p.cap * D;
+    const uint8_t* vb = p.v + bh * p.cap * D;
+    const uint8_t* ksb = p.ks + bh * p.nblk;
+    const uint8_t* vsb = p.vs + bh * p.nblk;
+    const int my_n = (n - warp + WARPS - 1) / WARPS;                  // tiles of this warp: warp, warp + 4, ...
+    const int key_first = (tl.x + ta + warp) * KT;
+
+    auto load_tile = [&](int i) {
+      const int key0 = key_first + i * (WARPS * KT);
+      const uint32_t dst = slot0 + (i % STAGES) * S::TILE;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int key = key0 + u * 16 + j * 8 + g;
+          const bool ok = key < kv_len;
+          const uint8_t* src = kb + (int64_t)(ok ? key : 0) * D + c * 16;
+#pragma unroll
+          for (int h = 0; h < HALVES; ++h)
+            cp16(dst + (u * 2 * HALVES + j * HALVES + h) * 512 + lane * 16, src + h * 64, ok);
+        }
+        const uint32_t vdst = dst + KT * D + u * 16 * D;
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4) {
+          const int key = key0 + u * 16 + (i4 >> 1) * 8 + 2 * c + (i4 & 1);
+          const bool ok = key < kv_len;
+          const uint8_t* src = vb + (int64_t)(ok ? key : 0) * D + g * VB;
+          if constexpr (D == 128) cp16(vdst + i4 * 512 + lane * 16, src, ok);
+          else cp_async_8(vdst + i4 * 256 + lane * 8, src, ok);
+        }
+      }
+    };
+    // scale bytes of a tile's keys: one a 16-key group, or one a key of this lane
+    constexpr int NS = UNI ? U : 4 * U;
+    int kbyte[NS], vbyte[NS];
+    auto load_scales = [&](int i, int (&kx)[NS], int (&vx)[NS]) {
+      const int key0 = key_first + i * (WARPS * KT);
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        const int key = UNI ? key0 + s * 16 : key0 + (s >> 2) * 16 + ((s >> 1) & 1) * 8 + 2 * c + (s & 1);
+        const bool ok = key < kv_len;
+        kx[s] = ok ? ksb[key >> p.shift] : kMinScale;
+        vx[s] = ok ? vsb[key >> p.shift] : kMinScale;
+      }
+    };
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) {
+      if (i < my_n) load_tile(i);
+      cp_commit();
+    }
+    if (my_n > 0) load_scales(0, kbyte, vbyte);
+
+    // ---- query rows g and g + 8 of the tile, scaled to f16
+    uint32_t qa[D / 16][4];
+    float rowf[2];
+    int qpos[2];
+#pragma unroll
+    for (int r2 = 0; r2 < 2; ++r2) {
+      const int r = rt * ROWS + g + r2 * 8;
+      const bool ok = r < rows_all;
+      const int gh = ok ? r / p.L : 0, i = ok ? r % p.L : 0;
+      qpos[r2] = kv_len - p.L + i;
+      const bf16* src = p.q + b * p.q_sb + i * p.q_st + (int64_t)(hk * G + gh) * p.q_sh + c * 16;
+      uint4 w[HALVES * 2];
+      uint32_t am = 0;
+#pragma unroll
+      for (int h = 0; h < HALVES * 2; ++h) {
+        w[h] = ok ? __ldg(reinterpret_cast<const uint4*>(src + (h >> 1) * 64 + (h & 1) * 8)) : make_uint4(0, 0, 0, 0);
+        am = __vmaxu2(am, __vmaxu2(w[h].x & 0x7fff7fffu, w[h].y & 0x7fff7fffu));
+        am = __vmaxu2(am, __vmaxu2(w[h].z & 0x7fff7fffu, w[h].w & 0x7fff7fffu));
+      }
+      uint32_t a16 = max(am & 0xffffu, am >> 16);
+      a16 = max(a16, __shfl_xor_sync(0xffffffffu, a16, 1));
+      a16 = max(a16, __shfl_xor_sync(0xffffffffu, a16, 2));
+      const int e = (int)(a16 >> 7);
+      // 2^(14 - (e - 127)); rows with an infinity or NaN keep their values (and give NaN)
+      const int field = e == 255 ? 127 : min(253, 268 - e);
+      const float mul = __int_as_float(field << 23) * p.sign;
+      rowf[r2] = __int_as_float((254 - field) << 23) * p.scale_log2;
+#pragma unroll
+      for (int h = 0; h < HALVES * 2; ++h) {
+        const uint32_t ww[4] = {w[h].x, w[h].y, w[h].z, w[h].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float x = __uint_as_float(ww[k] << 16) * mul, y = __uint_as_float(ww[k] & 0xffff0000u) * mul;
+          // elements (2k, 2k + 1) of 8: MMA step (k >> 1), its lower or upper k half
+          qa[h * 2 + (k >> 1)][(k & 1) * 2 + r2] = pack_f16(x, y);
+        }
+      }
+    }
+
+    float m[2] = {ninf, ninf}, l[2] = {0.f, 0.f};
+    float o[VB][4];
+#pragma unroll
+    for (int t = 0; t < VB; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+
+    for (int i = 0; i < my_n; ++i) {
+      if (i + STAGES - 1 < my_n) load_tile(i + STAGES - 1);
+      cp_commit();
+      int kx[NS], vx[NS];
+#pragma unroll
+      for (int s = 0; s < NS; ++s) kx[s] = kbyte[s], vx[s] = vbyte[s];
+      if (i + 1 < my_n) load_scales(i + 1, kbyte, vbyte);
+      cp_wait<STAGES - 1>();  // tile i has landed (a lane reads only what it copied itself)
+      const unsigned char* buf = ring + warp * (STAGES * S::TILE) + (i % STAGES) * S::TILE;
+      const int key0 = key_first + i * (WARPS * KT);
+      // ---- S = Q K^T
+      float s[2 * U][4];
+#pragma unroll
+      for (int j = 0; j < 2 * U; ++j) {
+        s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+#pragma unroll
+        for (int h = 0; h < HALVES; ++h) {
+          const uint4 w = *reinterpret_cast<const uint4*>(buf + (j * HALVES + h) * 512 + lane * 16);
+          const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint32_t b0, b1;
+            widen4<INT8>(ww[k], b0, b1);
+            mma_f16(s[j], qa[h * 4 + k], b0, b1);
+          }
+        }
+      }
+      // ---- t = s * f + log2 s_v, masked
+      float lv[NS], isv[NS];
+#pragma unroll
+      for (int x = 0; x < NS; ++x) {
+        lv[x] = vx[x] == kBadScale ? __int_as_float(0x7fffffff) : (float)(vx[x] - 127);
+        isv[x] = scale_inverse(min(vx[x], 253));
+      }
+      float f[2][NS];
+#pragma unroll
+      for (int x = 0; x < NS; ++x) {
+        const float sk = scale_value(kx[x]);
+        f[0][x] = rowf[0] * sk, f[1][x] = rowf[1] * sk;
+      }
+      // every row sees the whole tile
+      const bool inner = key0 + KT <= kv_len && (p.right < 0 || key0 + KT - 1 <= kv_len - p.L + p.right) &&
+                         (p.left < 0 || key0 >= kv_len - 1 - p.left);
+      float mx[2] = {ninf, ninf};
+#pragma unroll
+      for (int j = 0; j < 2 * U; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r2 = e >> 1, x = UNI ? j >> 1 : j * 2 + (e & 1);
+          s[j][e] = fmaf(s[j][e], f[r2][x], lv[x]);
+          if (!inner) {
+            const int key = key0 + j * 8 + 2 * c + (e & 1);
+            const bool vis = key < kv_len && (p.right < 0 || key <= qpos[r2] + p.right) &&
+                             (p.left < 0 || key >= qpos[r2] - p.left);
+            if (!vis) s[j][e] = ninf;
+          }
+          mx[r2] = fmaxf(mx[r2], s[j][e]);
+        }
+      // ---- follow the maximum; O is rescaled rarely
+      if (__any_sync(0xffffffffu, mx[0] > m[0] + 15.f || mx[1] > m[1] + 15.f)) {
+#pragma unroll
+        for (int r2 = 0; r2 < 2; ++r2) {
+          float x = mx[r2];
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+          const float to = x > m[r2] + 15.f ? x - 8.f : m[r2];
+          const float corr = to == m[r2] ? 1.f : ex2(m[r2] - to);
+          m[r2] = to;
+          l[r2] *= corr;
+#pragma unroll
+          for (int t = 0; t < VB; ++t) o[t][2 * r2] *= corr, o[t][2 * r2 + 1] *= corr;
+        }
+      }
+      const float mu[2] = {m[0] == ninf ? 0.f : m[0], m[1] == ninf ? 0.f : m[1]};
+#pragma unroll
+      for (int j = 0; j < 2 * U; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r2 = e >> 1, x = UNI ? j >> 1 : j * 2 + (e & 1);
+          s[j][e] = ex2(s[j][e] - mu[r2]);
+          l[r2] = fmaf(s[j][e], isv[x], l[r2]);
+        }
+      // ---- O += P V
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t pa[4] = {pack_f16(s[2 * u][0], s[2 * u][1]), pack_f16(s[2 * u][2], s[2 * u][3]),
+                                pack_f16(s[2 * u + 1][0], s[2 * u + 1][1]),
+                                pack_f16(s[2 * u + 1][2], s[2 * u + 1][3])};
+        uint32_t vw[4][VB / 4];
+        const unsigned char* vbuf = buf + KT * D + u * 16 * D;
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4) {
+          if constexpr (D == 128) {
+            const uint4 w = *reinterpret_cast<const uint4*>(vbuf + i4 * 512 + lane * 16);
+            vw[i4][0] = w.x, vw[i4][1] = w.y, vw[i4][2] = w.z, vw[i4][3] = w.w;
+          } else {
+            const uint2 w = *reinterpret_cast<const uint2*>(vbuf + i4 * 256 + lane * 8);
+            vw[i4][0] = w.x, vw[i4][1] = w.y;
+          }
+        }
+#pragma unroll
+        for (int x = 0; x < VB / 4; ++x) {
+          uint32_t b0[4], b1[4];  // f16 pairs of keys (2c, 2c + 1) and (2c + 8, 2c + 9) for columns 4x .. 4x + 3
+          widen4<INT8>(__byte_perm(vw[0][x], vw[1][x], 0x5140), b0[0], b0[1]);
+          widen4<INT8>(__byte_perm(vw[0][x], vw[1][x], 0x7362), b0[2], b0[3]);
+          widen4<INT8>(__byte_perm(vw[2][x], vw[3][x], 0x5140), b1[0], b1[1]);
+          widen4<INT8>(__byte_perm(vw[2][x], vw[3][x], 0x7362), b1[2], b1[3]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mma_f16(o[4 * x + k], pa, b0[k], b1[k]);
+        }
+      }
+    }
+    cp_wait<0>();
+#pragma unroll
+    for (int r2 = 0; r2 < 2; ++r2) {
+      l[r2] += __shfl_xor_sync(0xffffffffu, l[r2], 1);
+      l[r2] += __shfl_xor_sync(0xffffffffu, l[r2], 2);
+    }
+    // ---- join the warps through shared memory.  o[t][.] holds columns n = 2c, 2c + 1 of MMA tile t,
+    // which are head dims n * VB + t; kept as [row][t][n] until the end.
+    __syncthreads();
+    float* ow = reinterpret_cast<float*>(ring);
+    if (c == 0) {
+      wM[warp][g] = m[0], wM[warp][g + 8] = m[1];
+      wL[warp][g] = l[0], wL[warp][g + 8] = l[1];
+    }
+#pragma unroll
+    for (int t = 0; t < VB; ++t) {
+      float* dst = ow + (warp * ROWS + g) * S::OROW + t * 8 + 2 * c;
+      *reinterpret_cast<float2*>(dst) = make_float2(o[t][0], o[t][1]);
+      *reinterpret_cast<float2*>(dst + 8 * S::OROW) = make_float2(o[t][2], o[t][3]);
+    }
+    __syncthreads();
+    const bool whole = ta == 0 && n == nt;
+    const int slot = pos == first_of(blockIdx.x) ? 0 : 1;
+    float* part = p.part + ((int64_t)blockIdx.x * 2 + slot) * ROWS * D;
+    float* ml = p.ml + ((int64_t)blockIdx.x * 2 + slot) * ROWS * 2;
+    if (tid < ROWS) {
+      float M = wM[0][tid];
+      for (int w = 1; w < WARPS; ++w) M = fmaxf(M, wM[w][tid]);
+      float L = 0.f;
+      for (int w = 0; w < WARPS; ++w) {
+        const float fw = wM[w][tid] == ninf ? 0.f : ex2(wM[w][tid] - M);
+        // a warp without weight has l == 0; a NaN sum stays NaN
+        L += wL[w][tid] == 0.f ? 0.f : (wM[w][tid] == ninf ? 1.f : fw) * wL[w][tid];
+        wM[w][tid] = wL[w][tid] == 0.f ? 0.f : (wM[w][tid] == ninf ? 1.f : fw);
+      }
+      rM[tid] = M, rL[tid] = L;
+      if (!whole && tid < rows) ml[tid * 2] = M, ml[tid * 2 + 1] = L;
+    }
+    __syncthreads();
+    auto write_out = [&](int r, int tn, float x, float L) {  // tn = t * 8 + n
+      const int rr = rt * ROWS + r, gh = rr / p.L, i = rr % p.L;
+      p.o[(((int64_t)b * p.L + i) * p.H + hk * G + gh) * D + (tn & 7) * VB + (tn >> 3)] =
+          __float2bfloat16(L == 0.f ? 0.f : x / L);
+    };
+    for (int e = tid; e < rows * D; e += THREADS) {
+      const int r = e / D, tn = e % D;
+      float x = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w)
+        if (wM[w][r] != 0.f) x += wM[w][r] * ow[(w * ROWS + r) * S::OROW + tn];
+      if (whole) write_out(r, tn, x, rL[r]);
+      else part[e] = x;
+    }
+    if (!whole) {
+      // CTAs c0 .. c1 hold pieces of this column: those whose runs meet [c_first, c_first + nt)
+      const int64_t cf = base + (int64_t)col * nt, cl = cf + nt - 1;
+      auto owner = [&](int64_t at) {  // the CTA whose run holds position `at`
+        int64_t x = (at * active) / total;
+        while (first_of(x + 1) <= at) ++x;
+        while (first_of(x) > at) --x;
+        return (int)x;
+      };
+      const int c0 = owner(cf), c1 = owner(cl);
+      const int64_t cid = (int64_t)b * cols + col;
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) last = atomicAdd(&p.tickets[cid], 1) == c1 - c0;
+      __syncthreads();
+      if (last) {
+        __threadfence();
+        auto slot_of = [&](int x) { return x == c0 && first_of(x) != cf ? 1 : 0; };
+        if (tid < rows) {
+          float M = ninf;
+          for (int x = c0; x <= c1; ++x) M = fmaxf(M, __ldcg(p.ml + (((int64_t)x * 2 + slot_of(x)) * ROWS + tid) * 2));
+          float L = 0.f;
+          for (int x = c0; x <= c1; ++x) {
+            const float* q2 = p.ml + (((int64_t)x * 2 + slot_of(x)) * ROWS + tid) * 2;
+            const float mc = __ldcg(q2), lc = __ldcg(q2 + 1);
+            L += lc == 0.f ? 0.f : (mc == ninf ? 1.f : ex2(mc - M)) * lc;
+          }
+          rM[tid] = M, rL[tid] = L;
+        }
+        __syncthreads();
+        for (int e = tid; e < rows * D; e += THREADS) {
+          const int r = e / D;
+          float acc = 0.f;
+          for (int x = c0; x <= c1; ++x) {
+            const int64_t sl = (int64_t)x * 2 + slot_of(x);
+            const float* q2 = p.ml + (sl * ROWS + r) * 2;
+            const float mc = __ldcg(q2), lc = __ldcg(q2 + 1);
+            if (lc != 0.f) acc += (mc == ninf ? 1.f : ex2(mc - rM[r])) * __ldcg(p.part + sl * ROWS * D + e);
+          }
+          write_out(r, e % D, acc, rL[r]);
+        }
+      }
+    }
+    __syncthreads();  // the merge buffer is the ring
+    pos += n;
+  }
+}
+
+
+// Up to this many query rows a KV head (heads of the group x new tokens) take the kernel above,
+// whose 16-row tiles each walk the cache; more rows read the cache back to bf16 once and take
+// the prefill kernel.
+constexpr int kMaxRows = 64;
+
+}  // namespace kv8
+
+// q (B, L, H, D) bf16; new keys / values k, v (B, L, Hkv, D), if any, are written at
+// seqlens[b] first.  Queries are aligned to the end of the visible keys.
+torch::Tensor kv8_attend(torch::Tensor q, torch::Tensor keys, torch::Tensor values, torch::Tensor key_scales,
+                         torch::Tensor value_scales, int64_t block, c10::optional<torch::Tensor> k,
+                         c10::optional<torch::Tensor> v, torch::Tensor seqlens, double scale, int64_t left,
+                         int64_t right) {
+  using namespace kv8;
+  const char* who = "flash_attn_with_kvcache8";
+  c10::cuda::OptionalCUDAGuard guard;
+  if (keys.is_cuda()) guard.set_device(keys.device());
+  Cache c = check_cache(keys, values, key_scales, value_scales, block, who);
+  c.device = keys.get_device();
+  check_lens(seqlens, c, keys, who);
+  TORCH_CHECK(q.is_cuda() && q.get_device() == c.device && q.scalar_type() == at::kBFloat16 && q.dim() == 4 &&
+                  q.size(0) == c.B && q.size(3) == c.D,
+              who, ": queries (B, L, H, D) in bf16 on the cache's GPU");
+  TORCH_CHECK(k.has_value() == v.has_value(), who, ": new keys and values come together");
+  TORCH_CHECK(c.Hkv > 0 && q.size(2) % c.Hkv == 0, who, ": query heads (",
+              std::to_string(q.size(2)), ") must be a multiple of key/value heads (", std::to_string(c.Hkv), ")");
+  TORCH_CHECK(q.size(1) * q.size(2) <= (1 << 30), who, ": too many queries");
+  TORCH_CHECK(std::isfinite(scale), who, ": the softmax scale must be finite");
+  const int* lens = seqlens.data_ptr<int>();
+  int extra = 0;
+  if (k.has_value()) {
+    append(c, *k, *v, lens, who);
+    extra = (int)k->size(1);
+  }
+  const int L = (int)q.size(1), H = (int)q.size(2), G = H / c.Hkv;
+  auto o = torch::empty({c.B, L, H, c.D}, q.options());
+  if (o.numel() == 0) return o;
+  if (c.cap == 0) return o.zero_();
+  left = left < 0 ? -1 : std::min<int64_t>(left, 1 << 29);
+  right = right < 0 ? -1 : std::min<int64_t>(right, 1 << 29);
+  if ((int64_t)G * L > kMaxRows) {
+    auto opt = q.options();
+    auto kb = torch::empty({c.B, c.cap, c.Hkv, c.D}, opt), vb = torch::empty({c.B, c.cap, c.Hkv, c.D}, opt);
+    read(c, lens, extra, nullptr, 0, c.cap, 256, kb, vb, who);  // 256: more than a key tile of the prefill kernel
+    auto used = (seqlens + extra).clamp_(0, c.cap);
+    return fa_fwd(rows16(q) ? q : q.clone(at::MemoryFormat::Contiguous), kb, vb, c10::nullopt, c10::nullopt, used, L, c.cap, scale,
+                  left, right)[0];
+  }
+  if (!rows16(q)) q = q.clone(at::MemoryFormat::Contiguous);
+  AttendParams p{};
+  p.q = (const bf16*)q.data_ptr();
+  p.k = c.data[0], p.v = c.data[1], p.ks = c.scale[0], p.vs = c.scale[1];
+  p.seqlens = lens;
+  p.o = (bf16*)o.data_ptr();
+  p.q_sb = q.stride(0), p.q_st = q.stride(1), p.q_sh = q.stride(2);
+  p.B = c.B, p.L = L, p.H = H, p.Hkv = c.Hkv, p.RT = (G * L + ROWS - 1) / ROWS;
+  p.cap = c.cap, p.nblk = c.nblk, p.shift = c.shift, p.extra = extra;
+  p.left = (int)left, p.right = (int)right;
+  p.scale_log2 = (float)(std::abs(scale) * 1.4426950408889634), p.sign = scale < 0 ? -1.f : 1.f;
+  static int sms[64] = {0};
+  if (!sms[c.device]) C10_CUDA_CHECK(cudaDeviceGetAttribute(&sms[c.device], cudaDevAttrMultiProcessorCount, c.device));
+  const int per_sm = c.D == 64 ? Shape<64>::PER_SM : Shape<128>::PER_SM;
+  const int kt = c.D == 64 ? Shape<64>::KT : Shape<128>::KT;
+  int64_t span = c.cap;  // most keys a sequence can show
+  if (left >= 0) span = std::min<int64_t>(span, left + L + kt);
+  const int64_t columns = (int64_t)c.B * c.Hkv * p.RT;
+  const int64_t want = (columns * ((span + kt - 1) / kt) + WARPS - 1) / WARPS;
+  const int grid = (int)std::min<int64_t>(want, (int64_t)sms[c.device] * per_sm);
+  TORCH_CHECK(columns <= INT32_MAX / 4, who, ": too many sequences x heads");
+  // workspace: partials of at most two pieces a CTA, tickets of the columns (zeroed here)
+  const int64_t part = (int64_t)grid * 2 * ROWS * c.D, ml = (int64_t)grid * 2 * ROWS * 2;
+  auto work = torch::empty({part + ml + columns}, q.options().dtype(at::kFloat));
+  p.part = work.data_ptr<float>();
+  p.ml = p.part + part;
+  p.tickets = (int*)(p.ml + ml);
+  cudaStream_t st = at::cuda::getCurrentCUDAStream();
+  C10_CUDA_CHECK(cudaMemsetAsync(p.tickets, 0, columns * sizeof(int), st));
+  const bool uni = c.shift >= 4;
+  auto launch = [&](auto kern, SmemOptIn& attr, int smem) {
+    C10_CUDA_CHECK(attr.ensure(kern, smem));
+    kern<<<grid, THREADS, smem, st>>>(p);
+  };
+  static SmemOptIn a[8];
+#define KV8_CASE(d, i8, un) \
+  if (c.D == d && c.int8 == i8 && uni == un) \
+    launch(attend_kernel<d, i8, un>, a[(d == 128) * 4 + i8 * 2 + un], Shape<d>::SMEM)
+  KV8_CASE(64, false, false);
+  KV8_CASE(64, false, true);
+  KV8_CASE(64, true, false);
+  KV8_CASE(64, true, true);
+  KV8_CASE(128, false, false);
+  KV8_CASE(128, false, true);
+  KV8_CASE(128, true, false);
+  KV8_CASE(128, true, true);
+#undef KV8_CASE
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return o;
+}
+
+}  // namespace mykb

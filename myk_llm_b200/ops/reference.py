@@ -90,6 +90,73 @@ def attention_varlen_ref(q, k, v, cu_q, cu_k, causal=True, window=(-1, -1), soft
 
 
 # ---------------------------------------------------------------------------------------
+# 8-bit key/value cache
+# ---------------------------------------------------------------------------------------
+KV8_BAD = 255  # scale byte of a block that was given a NaN or an infinity
+
+
+def kv8_scale_byte(amax, int8):
+    """127 + log2 of the smallest power of two s with amax <= qmax * s (qmax 127 or 448), at
+    least 27; KV8_BAD where amax is not finite."""
+    m, e = torch.frexp(amax.float())
+    e = e + 127 - 7 + (m > 127 / 128) if int8 else e + 127 - 9 + (m > 448 / 512)
+    return torch.where(torch.isfinite(amax), e.clamp(min=27), torch.full_like(e, KV8_BAD))
+
+
+def kv8_scale(byte):
+    """2**(byte - 127) in fp32, NaN for KV8_BAD."""
+    byte = byte.int()
+    s = torch.ldexp(torch.ones_like(byte, dtype=torch.float32), byte.clamp(max=254) - 127)
+    return torch.where(byte == KV8_BAD, torch.full_like(s, math.nan), s)
+
+
+def kv8_round(x, dtype):
+    """fp32 values already divided by their scale -> 8-bit, ties to even (0 where NaN)."""
+    x = x.nan_to_num(0.0)
+    return x.round().clamp(-127, 127).to(dtype) if dtype == torch.int8 else x.clamp(-448, 448).to(dtype)
+
+
+def kv8_values(data, scales, block):
+    """fp32 values of a cache (B, H, cap, D) with scale bytes (B, H, blocks)."""
+    return data.float() * kv8_scale(scales).repeat_interleave(block, 2)[:, :, :data.shape[2], None]
+
+
+def kv8_append_ref(data, scales, block, x, seqlens):
+    """In place: x (B, new, H, D) at positions seqlens[b] onward of data (B, H, cap, D)."""
+    raw = data if data.dtype == torch.int8 else data.view(torch.uint8)  # indexable storage
+    for b, n in enumerate(seqlens.tolist()):
+        n = max(n, 0)
+        end = min(n + x.shape[1], data.shape[2])
+        for blk in range(n // block, -(-end // block)):
+            first = blk * block
+            lo, hi = max(n, first), min(end, first + block)
+            rows = x[b, lo - n:hi - n].transpose(0, 1).float()  # (H, rows, D)
+            byte = kv8_scale_byte(rows.abs().amax((1, 2)), data.dtype == torch.int8)
+            if lo > first:
+                old = scales[b, :, blk].int()
+                byte = torch.maximum(byte, old)
+                held = data[b, :, first:lo]
+                shift = torch.ldexp(torch.ones_like(byte, dtype=torch.float32), old - byte)[:, None, None]
+                moved = kv8_round(held.float() * shift, data.dtype).view(raw.dtype)
+                raw[b, :, first:lo] = torch.where((byte == KV8_BAD)[:, None, None], raw[b, :, first:lo], moved)
+            scales[b, :, blk] = byte.to(torch.uint8)
+            raw[b, :, lo:hi] = kv8_round(rows / kv8_scale(byte)[:, None, None], data.dtype).view(raw.dtype)
+
+
+def kv8_read_ref(data, scales, block, seqlens, start, length):
+    """bf16 (B, length, H, D) of positions start (int or (B)) onward, 0 from seqlens[b] on."""
+    cap = data.shape[2]
+    out = torch.zeros(data.shape[0], length, data.shape[1], data.shape[3], dtype=torch.bfloat16, device=data.device)
+    values = kv8_values(data, scales, block)
+    for b, n in enumerate(seqlens.tolist()):
+        s = int(start[b]) if isinstance(start, torch.Tensor) else start
+        lo, hi = max(s, 0), min(s + length, n, cap)
+        if lo < hi:
+            out[b, lo - s:hi - s] = values[b, :, lo:hi].transpose(0, 1).to(torch.bfloat16)
+    return out
+
+
+# ---------------------------------------------------------------------------------------
 # elementwise / normalisation
 # ---------------------------------------------------------------------------------------
 def rms_norm_ref(x, weight, eps):
@@ -141,6 +208,26 @@ def linear_cross_entropy_ref(hidden, weight, targets, normalizer, z_loss=0.0):
     ce_sum, z_sum = ce.sum(), z.sum()
     loss = (ce_sum + z_loss * z_sum) / normalizer
     return loss, ce_sum.detach(), z_sum.detach()
+
+
+def token_logprobs_ref(logits, tokens, top, ignore_index=IGNORE_INDEX):
+    """(logprobs, entropy, top_logprobs, top_tokens) of logits (..., V), in fp32 (fp64 for fp64
+    logits)."""
+    x = logits if logits.dtype == torch.float64 else logits.float()
+    vocab = x.shape[-1]
+    empty = (x == -math.inf).all(-1)
+    none = empty[..., None].expand_as(x)
+    lse = torch.logsumexp(torch.where(none, torch.zeros_like(x), x), -1, keepdim=True)
+    z = torch.where(none, torch.full_like(x, -math.inf), x - lse)
+    out_of_range = (tokens < 0) | (tokens >= vocab)
+    lp = z.gather(-1, tokens.long().clamp(0, vocab - 1)[..., None])[..., 0]
+    lp = torch.where(out_of_range, torch.full_like(lp, math.nan), lp)
+    lp = torch.where(tokens == ignore_index, torch.zeros_like(lp), lp)
+    finite = torch.where(z < -1e4, torch.zeros_like(z), z)  # 0 log 0 is 0
+    entropy = torch.where(empty, torch.zeros_like(lp), -(z.exp() * finite).sum(-1))
+    ranked = torch.where(torch.isnan(x), torch.full_like(x, -math.inf), x).detach()
+    order = torch.sort(ranked, dim=-1, descending=True, stable=True).indices[..., :top].contiguous()
+    return lp, entropy, z.gather(-1, order), order
 
 
 # ---------------------------------------------------------------------------------------
