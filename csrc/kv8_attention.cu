@@ -19,9 +19,9 @@
 // MMAs into its own slots of shared memory (cp.async, several tiles ahead), so there are no
 // bank conflicts, barriers or transposes: the contraction index of Q K^T and the column index
 // of P V are permuted to make a lane's bytes contiguous in memory.
-// A column that one CTA covers is written at once; else the CTAs leave fp32 partials and the
-// last one to finish (a ticket; nothing waits) joins them in order, so results do not depend
-// on timing.
+// A column that one CTA covers is written at once; else the CTAs leave fp32 partials and a
+// second kernel, whose start overlaps the first, joins them in order: no atomics, and results
+// that do not depend on timing.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -47,9 +47,9 @@ struct AttendParams {
   const uint8_t* vs;
   const int* seqlens;  // (B)
   bf16* o;             // (B, L, H, D) contiguous
-  float* part;         // [grid][2][rows <= 16][D] partial O, columns permuted (see flush)
-  float* ml;           // [grid][2][16][2]
-  int* tickets;        // [B * Hkv * RT], zero
+  float* part;         // [grid][2][16][D] partial O of a CTA's first and last piece, as [row][t][n] (see attend_kernel)
+  float* ml;           // [grid][2][16][2] their maxima and sums
+  int grid;            // CTAs of attend_kernel
   int64_t q_sb, q_st, q_sh;
   int B, L, H, Hkv, RT, cap, nblk, shift;
   int extra;           // visible keys = seqlens + extra
@@ -82,6 +82,16 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
+// Lets the next kernel of the stream start its prologue; waits until the one before has finished
+// (both do nothing where the kernel was launched without that attribute).
+__device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;"); }
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Weight of a partial (m, l) when joined under the maximum M: 0 without any weight; a sum that is
+// not a number stays one.
+__device__ __forceinline__ float part_weight(float m, float l, float M) {
+  return l == 0.f ? 0.f : m == -INFINITY ? 1.f : ex2(m - M);
+}
+
 // Shape of the kernel for one head_dim: keys a tile, tiles in the ring, CTAs an SM.
 template <int D>
 struct Shape {
@@ -104,36 +114,64 @@ __device__ __forceinline__ int2 tiles_of(const AttendParams& p, int b, int& kv_l
   return make_int2(t0, (kv_len + KT - 1) / KT - t0);
 }
 
+// The work list: `total` tiles in runs of `per` or, for the first `rem` CTAs, per + 1.
+struct Runs {
+  int total, active, per, rem;
+  __device__ __forceinline__ Runs(int total_, int grid) {
+    total = total_;
+    // as many CTAs take part as get at least one tile a warp
+    active = max(1, min(grid, (total + WARPS - 1) / WARPS));
+    per = total / active, rem = total - per * active;
+  }
+  __device__ __forceinline__ int first(int cta) const { return cta * per + min(cta, rem); }
+  __device__ __forceinline__ int owner(int at) const {
+    const int cut = rem * (per + 1);
+    return at < cut ? at / (per + 1) : rem + (at - cut) / per;
+  }
+};
+
+__device__ __forceinline__ int block_sum(int x, int* red) {  // of all THREADS threads, to all of them
+  x = __reduce_add_sync(0xffffffffu, x);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = x;
+  __syncthreads();
+  x = 0;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) x += red[w];
+  __syncthreads();
+  return x;
+}
+
+// o of row r of a 16-row tile: where its D outputs start
+__device__ __forceinline__ bf16* out_row(const AttendParams& p, int b, int hk, int row, int D) {
+  const int g = row / p.L, i = row - g * p.L;
+  return p.o + (((int64_t)b * p.L + i) * p.H + hk * (p.H / p.Hkv) + g) * D;
+}
+
 // UNI: a scale block spans whole 16-key groups (block >= 16), else each key has its own lookup.
 template <int D, bool INT8, bool UNI>
 __global__ void __launch_bounds__(THREADS, Shape<D>::PER_SM) attend_kernel(AttendParams p) {
   using S = Shape<D>;
   constexpr int KT = S::KT, STAGES = S::STAGES, U = KT / 16, HALVES = D / 64, VB = D / 8;
   extern __shared__ __align__(128) unsigned char ring[];
-  __shared__ int64_t scan[THREADS + 1];
-  __shared__ int64_t start_base;
-  __shared__ int start_b, last;
-  __shared__ float wM[WARPS][ROWS], wL[WARPS][ROWS], rM[ROWS], rL[ROWS];
+  __shared__ int scan[THREADS + 1];
+  __shared__ int start_base, start_b;
+  __shared__ float wM[WARPS][ROWS], wL[WARPS][ROWS], rL[ROWS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int G = p.H / p.Hkv, rows_all = G * p.L;
   const int cols = p.Hkv * p.RT;  // columns a sequence
+  launch_dependents();
 
   // ---- the work list: each thread sums a run of sequences, then a scan over the threads
   const int run = (p.B + THREADS - 1) / THREADS;
-  int64_t mine = 0;
-  for (int i = 0; i < run; ++i) {
-    const int b = tid * run + i;
-    int kl;
-    if (b < p.B) mine += tiles_of<KT>(p, b, kl).y;
-  }
   {
-    int64_t x = mine;
+    int x = 0, kl;
+    for (int i = tid * run; i < min((tid + 1) * run, p.B); ++i) x += tiles_of<KT>(p, i, kl).y;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
-    __shared__ int64_t wsum[WARPS];
+    __shared__ int wsum[WARPS];
     if (lane == 31) wsum[warp] = x;
     __syncthreads();
     for (int w = 0; w < warp; ++w) x += wsum[w];
@@ -141,9 +179,18 @@ __global__ void __launch_bounds__(THREADS, Shape<D>::PER_SM) attend_kernel(Atten
     if (tid == 0) scan[0] = 0;
     __syncthreads();
   }
-  const int64_t total = scan[THREADS] * cols;
-  // as many CTAs take part as get at least one tile a warp
-  const int64_t active = min((int64_t)gridDim.x, (total + WARPS - 1) / WARPS);
+  const Runs runs(scan[THREADS] * cols, gridDim.x);
+  int pos = runs.first(blockIdx.x);
+  const int run_first = pos, end = blockIdx.x < runs.active ? runs.first(blockIdx.x + 1) : pos;
+  if (scan[tid] * cols <= pos && pos < scan[tid + 1] * cols) {
+    int base = scan[tid] * cols, b = tid * run, kl;
+    for (;; ++b) {
+      const int n = tiles_of<KT>(p, b, kl).y * cols;
+      if (pos < base + n) break;
+      base += n;
+    }
+    start_b = b, start_base = base;
+  }
   // sequences without visible keys: their rows are 0
   for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
     int kl;
@@ -151,24 +198,10 @@ __global__ void __launch_bounds__(THREADS, Shape<D>::PER_SM) attend_kernel(Atten
     uint32_t* o = reinterpret_cast<uint32_t*>(p.o + (int64_t)b * p.L * p.H * D);
     for (int64_t i = tid; i < (int64_t)p.L * p.H * D / 2; i += THREADS) o[i] = 0;
   }
-  if (blockIdx.x >= active) return;
-  auto first_of = [&](int64_t cta) { return total * cta / active; };
-  int64_t pos = first_of(blockIdx.x);
-  const int64_t end = first_of(blockIdx.x + 1);
-  if (scan[tid] * cols <= pos && pos < scan[tid + 1] * cols) {
-    int64_t base = scan[tid] * cols;
-    int b = tid * run;
-    for (;; ++b) {
-      int kl;
-      const int64_t n = (int64_t)tiles_of<KT>(p, b, kl).y * cols;
-      if (pos < base + n) break;
-      base += n;
-    }
-    start_b = b, start_base = base;
-  }
+  grid_dependency_wait();  // the new tokens are in the cache
+  if (pos >= end) return;
   __syncthreads();
-  int b = start_b;
-  int64_t base = start_base;
+  int b = start_b, base = start_base;
   const uint32_t slot0 = smem_u32(ring) + warp * (STAGES * S::TILE);
   const float ninf = -INFINITY;
 
@@ -176,15 +209,15 @@ __global__ void __launch_bounds__(THREADS, Shape<D>::PER_SM) attend_kernel(Atten
     int kv_len;
     const int2 tl = tiles_of<KT>(p, b, kv_len);
     const int nt = tl.y;
-    if (pos >= base + (int64_t)nt * cols) {
-      base += (int64_t)nt * cols;
+    if (pos >= base + nt * cols) {
+      base += nt * cols;
       ++b;
       continue;
     }
-    const int col = (int)((pos - base) / nt);
-    const int ta = (int)((pos - base) - (int64_t)col * nt);          // first tile of this piece
-    const int n = (int)min((int64_t)(nt - ta), end - pos);            // its tiles
-    const int hk = col / p.RT, rt = col % p.RT;
+    const int col = (pos - base) / nt;
+    const int ta = (pos - base) - col * nt;    // first tile of this piece
+    const int n = min(nt - ta, end - pos);     // its tiles
+    const int hk = col / p.RT, rt = col - hk * p.RT;
     const int rows = min(ROWS, rows_all - rt * ROWS);
     const int64_t bh = (int64_t)b * p.Hkv + hk;
     const uint8_t* kb = p.k + bh * p.cap * D;
@@ -417,78 +450,43 @@ __global__ void __launch_bounds__(THREADS, Shape<D>::PER_SM) attend_kernel(Atten
     }
     __syncthreads();
     const bool whole = ta == 0 && n == nt;
-    const int slot = pos == first_of(blockIdx.x) ? 0 : 1;
-    float* part = p.part + ((int64_t)blockIdx.x * 2 + slot) * ROWS * D;
-    float* ml = p.ml + ((int64_t)blockIdx.x * 2 + slot) * ROWS * 2;
+    const int64_t slot = (int64_t)blockIdx.x * 2 + (pos != run_first);
     if (tid < ROWS) {
       float M = wM[0][tid];
+#pragma unroll
       for (int w = 1; w < WARPS; ++w) M = fmaxf(M, wM[w][tid]);
       float L = 0.f;
+#pragma unroll
       for (int w = 0; w < WARPS; ++w) {
-        const float fw = wM[w][tid] == ninf ? 0.f : ex2(wM[w][tid] - M);
-        // a warp without weight has l == 0; a NaN sum stays NaN
-        L += wL[w][tid] == 0.f ? 0.f : (wM[w][tid] == ninf ? 1.f : fw) * wL[w][tid];
-        wM[w][tid] = wL[w][tid] == 0.f ? 0.f : (wM[w][tid] == ninf ? 1.f : fw);
+        const float f = part_weight(wM[w][tid], wL[w][tid], M);
+        L += f == 0.f ? 0.f : f * wL[w][tid];
+        wM[w][tid] = f;
       }
-      rM[tid] = M, rL[tid] = L;
-      if (!whole && tid < rows) ml[tid * 2] = M, ml[tid * 2 + 1] = L;
+      rL[tid] = L;
+      if (!whole && tid < rows) *reinterpret_cast<float2*>(p.ml + (slot * ROWS + tid) * 2) = make_float2(M, L);
     }
     __syncthreads();
-    auto write_out = [&](int r, int tn, float x, float L) {  // tn = t * 8 + n
-      const int rr = rt * ROWS + r, gh = rr / p.L, i = rr % p.L;
-      p.o[(((int64_t)b * p.L + i) * p.H + hk * G + gh) * D + (tn & 7) * VB + (tn >> 3)] =
-          __float2bfloat16(L == 0.f ? 0.f : x / L);
-    };
-    for (int e = tid; e < rows * D; e += THREADS) {
-      const int r = e / D, tn = e % D;
-      float x = 0.f;
+    for (int e = tid; e < rows * VB; e += THREADS) {  // (row, t): n = 0 .. 7
+      const int r = e / VB, t = e % VB;
+      float x[8] = {};
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w)
-        if (wM[w][r] != 0.f) x += wM[w][r] * ow[(w * ROWS + r) * S::OROW + tn];
-      if (whole) write_out(r, tn, x, rL[r]);
-      else part[e] = x;
-    }
-    if (!whole) {
-      // CTAs c0 .. c1 hold pieces of this column: those whose runs meet [c_first, c_first + nt)
-      const int64_t cf = base + (int64_t)col * nt, cl = cf + nt - 1;
-      auto owner = [&](int64_t at) {  // the CTA whose run holds position `at`
-        int64_t x = (at * active) / total;
-        while (first_of(x + 1) <= at) ++x;
-        while (first_of(x) > at) --x;
-        return (int)x;
-      };
-      const int c0 = owner(cf), c1 = owner(cl);
-      const int64_t cid = (int64_t)b * cols + col;
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) last = atomicAdd(&p.tickets[cid], 1) == c1 - c0;
-      __syncthreads();
-      if (last) {
-        __threadfence();
-        auto slot_of = [&](int x) { return x == c0 && first_of(x) != cf ? 1 : 0; };
-        if (tid < rows) {
-          float M = ninf;
-          for (int x = c0; x <= c1; ++x) M = fmaxf(M, __ldcg(p.ml + (((int64_t)x * 2 + slot_of(x)) * ROWS + tid) * 2));
-          float L = 0.f;
-          for (int x = c0; x <= c1; ++x) {
-            const float* q2 = p.ml + (((int64_t)x * 2 + slot_of(x)) * ROWS + tid) * 2;
-            const float mc = __ldcg(q2), lc = __ldcg(q2 + 1);
-            L += lc == 0.f ? 0.f : (mc == ninf ? 1.f : ex2(mc - M)) * lc;
-          }
-          rM[tid] = M, rL[tid] = L;
-        }
-        __syncthreads();
-        for (int e = tid; e < rows * D; e += THREADS) {
-          const int r = e / D;
-          float acc = 0.f;
-          for (int x = c0; x <= c1; ++x) {
-            const int64_t sl = (int64_t)x * 2 + slot_of(x);
-            const float* q2 = p.ml + (sl * ROWS + r) * 2;
-            const float mc = __ldcg(q2), lc = __ldcg(q2 + 1);
-            if (lc != 0.f) acc += (mc == ninf ? 1.f : ex2(mc - rM[r])) * __ldcg(p.part + sl * ROWS * D + e);
-          }
-          write_out(r, e % D, acc, rL[r]);
-        }
+      for (int w = 0; w < WARPS; ++w) {
+        const float f = wM[w][r];
+        if (f == 0.f) continue;
+        const float4* src = reinterpret_cast<const float4*>(ow + (w * ROWS + r) * S::OROW + t * 8);
+        const float4 u = src[0], v = src[1];
+        x[0] += f * u.x, x[1] += f * u.y, x[2] += f * u.z, x[3] += f * u.w;
+        x[4] += f * v.x, x[5] += f * v.y, x[6] += f * v.z, x[7] += f * v.w;
+      }
+      if (whole) {
+        bf16* o = out_row(p, b, hk, rt * ROWS + r, D) + t;
+        const float inv = rL[r] == 0.f ? 0.f : 1.f / rL[r];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) o[k * VB] = __float2bfloat16(x[k] * inv);
+      } else {
+        float4* dst = reinterpret_cast<float4*>(p.part + (slot * ROWS + r) * D + t * 8);
+        dst[0] = make_float4(x[0], x[1], x[2], x[3]);
+        dst[1] = make_float4(x[4], x[5], x[6], x[7]);
       }
     }
     __syncthreads();  // the merge buffer is the ring
@@ -496,6 +494,89 @@ __global__ void __launch_bounds__(THREADS, Shape<D>::PER_SM) attend_kernel(Atten
   }
 }
 
+// Joins the partials of the columns that several CTAs share, in the order of the CTAs; one CTA a
+// column.  Launched so that everything up to the wait overlaps attend_kernel.
+template <int D>
+__global__ void __launch_bounds__(THREADS) join_kernel(AttendParams p) {
+  constexpr int KT = Shape<D>::KT, VB = D / 8, D4 = D / 4, MAXE = ROWS * D4 / THREADS;
+  extern __shared__ float wt[];  // [partials][ROWS] weights
+  __shared__ int red[WARPS];
+  __shared__ float sL[ROWS];
+  __shared__ float4 part[THREADS];
+  const int tid = threadIdx.x;
+  const int cols = p.Hkv * p.RT;
+  const int b = blockIdx.x / cols, col = blockIdx.x - b * cols;
+  int kl, all = 0, before = 0;
+  for (int i = tid; i < p.B; i += THREADS) {
+    const int n = tiles_of<KT>(p, i, kl).y;
+    all += n;
+    if (i < b) before += n;
+  }
+  const Runs runs(block_sum(all, red) * cols, p.grid);
+  const int nt = tiles_of<KT>(p, b, kl).y;
+  const int cf = block_sum(before, red) * cols + col * nt;
+  grid_dependency_wait();
+  if (nt == 0) return;
+  const int c0 = runs.owner(cf), nc = runs.owner(cf + nt - 1) + 1 - c0;
+  if (nc == 1) return;  // written by attend_kernel
+  const int hk = col / p.RT, rt = col - hk * p.RT;
+  const int rows = min(ROWS, (p.H / p.Hkv) * p.L - rt * ROWS);
+  // the column is the first piece of every CTA but c0, and of c0 only if c0's run starts with it
+  const bool late = runs.first(c0) != cf;
+  auto slot = [&](int x) { return ((int64_t)c0 + x) * 2 + (x == 0 && late); };
+  {  // rows' maxima, weights and sums: 8 threads a row
+    const int r = tid >> 3;
+    float M = -INFINITY, L = 0.f;
+    if (r < rows)
+      for (int x = tid & 7; x < nc; x += 8) M = fmaxf(M, __ldcg(p.ml + (slot(x) * ROWS + r) * 2));
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    if (r < rows)
+      for (int x = tid & 7; x < nc; x += 8) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.ml + (slot(x) * ROWS + r) * 2));
+        const float f = part_weight(ml.x, ml.y, M);
+        wt[x * ROWS + r] = f;
+        if (f != 0.f) L += f * ml.y;
+      }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    if ((tid & 7) == 0) sL[r] = L;
+  }
+  __syncthreads();
+  // O as float4 columns; with few rows, groups of threads take every groups-th partial
+  const int n4 = rows * D4, groups = n4 >= THREADS ? 1 : THREADS / n4;
+#pragma unroll
+  for (int k = 0; k < MAXE; ++k) {
+    if (k * THREADS >= n4) break;
+    const int e = groups > 1 ? tid % n4 : k * THREADS + tid, first = groups > 1 ? tid / n4 : 0;
+    const int r = e / D4;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (e < n4 && first < groups) {
+#pragma unroll 8
+      for (int x = first; x < nc; x += groups) {
+        const float f = wt[x * ROWS + r];
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part + slot(x) * ROWS * D) + e);
+        if (f != 0.f) a.x += f * v.x, a.y += f * v.y, a.z += f * v.z, a.w += f * v.w;
+      }
+    }
+    if (groups > 1) {
+      part[tid] = a;
+      __syncthreads();
+      if (tid < n4)
+        for (int x = 1; x < groups; ++x) {
+          const float4 v = part[x * n4 + tid];
+          a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+        }
+    }
+    if (groups > 1 ? tid < n4 : e < n4) {
+      const int tn = (e % D4) * 4;
+      bf16* o = out_row(p, b, hk, rt * ROWS + r, D) + (tn & 7) * VB + (tn >> 3);
+      const float inv = sL[r] == 0.f ? 0.f : 1.f / sL[r];
+      o[0] = __float2bfloat16(a.x * inv), o[VB] = __float2bfloat16(a.y * inv);
+      o[2 * VB] = __float2bfloat16(a.z * inv), o[3 * VB] = __float2bfloat16(a.w * inv);
+    }
+  }
+}
 
 // Up to this many query rows a KV head (heads of the group x new tokens) take the kernel above,
 // whose 16-row tiles each walk the cache; more rows read the cache back to bf16 once and take
@@ -565,19 +646,27 @@ torch::Tensor kv8_attend(torch::Tensor q, torch::Tensor keys, torch::Tensor valu
   const int64_t columns = (int64_t)c.B * c.Hkv * p.RT;
   const int64_t want = (columns * ((span + kt - 1) / kt) + WARPS - 1) / WARPS;
   const int grid = (int)std::min<int64_t>(want, (int64_t)sms[c.device] * per_sm);
-  TORCH_CHECK(columns <= INT32_MAX / 4, who, ": too many sequences x heads");
-  // workspace: partials of at most two pieces a CTA, tickets of the columns (zeroed here)
+  TORCH_CHECK(columns * ((c.cap + kt - 1) / kt) <= INT32_MAX, who, ": too many sequences x heads x keys");
+  // workspace: partials of at most two pieces a CTA
   const int64_t part = (int64_t)grid * 2 * ROWS * c.D, ml = (int64_t)grid * 2 * ROWS * 2;
-  auto work = torch::empty({part + ml + columns}, q.options().dtype(at::kFloat));
+  auto work = torch::empty({part + ml}, q.options().dtype(at::kFloat));
   p.part = work.data_ptr<float>();
   p.ml = p.part + part;
-  p.tickets = (int*)(p.ml + ml);
+  p.grid = grid;
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
-  C10_CUDA_CHECK(cudaMemsetAsync(p.tickets, 0, columns * sizeof(int), st));
+  auto start = [&](auto kern, int blocks, int smem, bool overlap) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = blocks, cfg.blockDim = THREADS, cfg.dynamicSmemBytes = smem, cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr, cfg.numAttrs = overlap ? 1 : 0;
+    C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, p));
+  };
   const bool uni = c.shift >= 4;
   auto launch = [&](auto kern, SmemOptIn& attr, int smem) {
     C10_CUDA_CHECK(attr.ensure(kern, smem));
-    kern<<<grid, THREADS, smem, st>>>(p);
+    start(kern, grid, smem, extra > 0);  // the kernel before it is then append()'s
   };
   static SmemOptIn a[8];
 #define KV8_CASE(d, i8, un) \
@@ -592,7 +681,9 @@ torch::Tensor kv8_attend(torch::Tensor q, torch::Tensor keys, torch::Tensor valu
   KV8_CASE(128, true, false);
   KV8_CASE(128, true, true);
 #undef KV8_CASE
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  const int weights = grid * ROWS * (int)sizeof(float);
+  if (c.D == 64) start(join_kernel<64>, (int)columns, weights, true);
+  else start(join_kernel<128>, (int)columns, weights, true);
   return o;
 }
 

@@ -28,6 +28,8 @@ constexpr int kAppendWarps = 4, kHeld = 8;
 
 template <int D, bool INT8>
 __global__ void __launch_bounds__(kAppendWarps * 32) append_kernel(AppendParams p) {
+  // a kernel that attends to the new tokens may start its prologue (and waits for the rest)
+  asm volatile("griddepcontrol.launch_dependents;");
   const int lane = threadIdx.x & 31;
   int64_t u = (int64_t)blockIdx.x * kAppendWarps + (threadIdx.x >> 5);
   if (u >= (int64_t)p.B * p.Hkv * p.span * 2) return;
