@@ -15,10 +15,11 @@
 // bound by HBM.  One work list holds the 16-key-multiple tiles of all (sequence, KV head,
 // 16-row tile) columns; every CTA takes an equal run of it, computed on the device from the
 // lengths (ragged batches stay balanced, a captured CUDA graph stays valid).  The four warps
-// of a CTA take its tiles in turn; each lane copies exactly the bytes that it will feed to the
-// MMAs into its own slots of shared memory (cp.async, several tiles ahead), so there are no
-// bank conflicts, barriers or transposes: the contraction index of Q K^T and the column index
-// of P V are permuted to make a lane's bytes contiguous in memory.
+// of a CTA take its tiles in turn, each through a ring of its own that TMA fills (32 keys and 32
+// values, two bulk copies), so they never wait for one another inside a column.  Keys are the M
+// side of Q K^T and head dims that of P V, so that one 8-column tile holds up to 8 query rows;
+// the contraction index of the first and the row index of the second are permuted to make a
+// lane's bytes contiguous in shared memory.
 // A column that one CTA covers is written at once; else the CTAs leave fp32 partials and a
 // second kernel, whose start overlaps the first, joins them in order: no atomics, and results
 // that do not depend on timing.
@@ -28,6 +29,7 @@
 
 #include "kv8.cuh"
 #include "kv8_host.h"
+#include "tma_host.h"
 
 namespace mykb {
 std::vector<torch::Tensor> fa_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, c10::optional<torch::Tensor> cu_q,
@@ -35,21 +37,20 @@ std::vector<torch::Tensor> fa_fwd(torch::Tensor q, torch::Tensor k, torch::Tenso
                                   int64_t max_q, int64_t max_k, double scale, int64_t left, int64_t right);
 namespace kv8 {
 
-constexpr int ROWS = 16;   // query rows of one MMA tile
 constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
+constexpr int KT = 32;        // keys of a tile
 
 struct AttendParams {
   const bf16* q;       // (B, L, H, D)
-  const uint8_t* k;    // (B, Hkv, cap, D)
-  const uint8_t* v;
   const uint8_t* ks;   // (B, Hkv, nblk)
   const uint8_t* vs;
   const int* seqlens;  // (B)
   bf16* o;             // (B, L, H, D) contiguous
-  float* part;         // [grid][2][16][D] partial O of a CTA's first and last piece, as [row][t][n] (see attend_kernel)
-  float* ml;           // [grid][2][16][2] their maxima and sums
+  float* part;         // [grid][2][rows][D] partial O of a CTA's first and last piece
+  float* ml;           // [grid][2][rows][2] their maxima and sums
   int grid;            // CTAs of attend_kernel
+  int* status;
   int64_t q_sb, q_st, q_sh;
   int B, L, H, Hkv, RT, cap, nblk, shift;
   int extra;           // visible keys = seqlens + extra
@@ -58,14 +59,6 @@ struct AttendParams {
   float sign;
 };
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
-}
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -77,6 +70,12 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+// 8 x 8 transpose of 16-bit elements over the warp: lane (g, c) gives row g, columns 2c and 2c + 1.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&h);
@@ -86,26 +85,29 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 // (both do nothing where the kernel was launched without that attribute).
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;"); }
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// A tile has landed.  If it does not within a second, the status word says so and the kernel winds down.
+__device__ __forceinline__ void tile_wait(uint64_t* bar, uint32_t parity, int* status) {
+  if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) mbar_wait_warp(bar, parity, status, __LINE__);
+}
 // Weight of a partial (m, l) when joined under the maximum M: 0 without any weight; a sum that is
 // not a number stays one.
 __device__ __forceinline__ float part_weight(float m, float l, float M) {
   return l == 0.f ? 0.f : m == -INFINITY ? 1.f : ex2(m - M);
 }
 
-// Shape of the kernel for one head_dim: keys a tile, tiles in the ring, CTAs an SM.
-template <int D>
+// Shape of the kernel for one head_dim and NT 8-query tiles: keys a tile, tiles in the ring of a
+// warp, CTAs an SM.
+template <int D, int NT>
 struct Shape {
-  static constexpr int KT = 32;
-  static constexpr int STAGES = 3;
+  static constexpr int ROWS = 8 * NT;
+  static constexpr int STAGES = D == 64 ? 3 : 1 + NT;
+  static constexpr int PER_SM = (D == 64 ? 4 : 3) - (NT - 1);
   static constexpr int TILE = KT * D * 2;  // bytes of a tile's keys and values
   static constexpr int RING = WARPS * STAGES * TILE;
-  static constexpr int OROW = D + 8;       // floats of a row in the merge buffer: conflict-free float2 writes
+  static constexpr int OROW = D + 4;       // floats of a row in the merge buffer
   static constexpr int SMEM = RING > WARPS * ROWS * OROW * 4 ? RING : WARPS * ROWS * OROW * 4;
-  static constexpr int PER_SM = D == 64 ? 3 : 2;
 };
-
 // Tiles of a sequence that some query sees: [t0, t0 + n).
-template <int KT>
 __device__ __forceinline__ int2 tiles_of(const AttendParams& p, int b, int& kv_len) {
   kv_len = (int)min((int64_t)max(p.seqlens[b], 0) + p.extra, (int64_t)p.cap);
   if (kv_len <= 0) return make_int2(0, 0);
@@ -148,11 +150,13 @@ __device__ __forceinline__ bf16* out_row(const AttendParams& p, int b, int hk, i
 }
 
 // UNI: a scale block spans whole 16-key groups (block >= 16), else each key has its own lookup.
-template <int D, bool INT8, bool UNI>
-__global__ void __launch_bounds__(THREADS, Shape<D>::PER_SM) attend_kernel(AttendParams p) {
-  using S = Shape<D>;
-  constexpr int KT = S::KT, STAGES = S::STAGES, U = KT / 16, HALVES = D / 64, VB = D / 8;
-  extern __shared__ __align__(128) unsigned char ring[];
+template <int D, int NT, bool INT8, bool UNI>
+__global__ void __launch_bounds__(THREADS, Shape<D, NT>::PER_SM)
+attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv, AttendParams p) {
+  using S = Shape<D, NT>;
+  constexpr int STAGES = S::STAGES, ROWS = S::ROWS, U = KT / 16, HALVES = D / 64, VB = D / 8, MT = D / 16;
+  extern __shared__ __align__(1024) unsigned char ring[];
+  __shared__ uint64_t full[WARPS][STAGES];
   __shared__ int scan[THREADS + 1];
   __shared__ int start_base, start_b;
   __shared__ float wM[WARPS][ROWS], wL[WARPS][ROWS], rL[ROWS];
@@ -160,12 +164,19 @@ __global__ void __launch_bounds__(THREADS, Shape<D>::PER_SM) attend_kernel(Atten
   const int G = p.H / p.Hkv, rows_all = G * p.L;
   const int cols = p.Hkv * p.RT;  // columns a sequence
   launch_dependents();
+  if (lane == 0) {
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i) mbar_init(&full[warp][i], 1);
+    fence_barrier_init();
+    tma_prefetch_desc(&tmk);
+    tma_prefetch_desc(&tmv);
+  }
 
   // ---- the work list: each thread sums a run of sequences, then a scan over the threads
   const int run = (p.B + THREADS - 1) / THREADS;
   {
     int x = 0, kl;
-    for (int i = tid * run; i < min((tid + 1) * run, p.B); ++i) x += tiles_of<KT>(p, i, kl).y;
+    for (int i = tid * run; i < min((tid + 1) * run, p.B); ++i) x += tiles_of(p, i, kl).y;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, x, o);
@@ -185,7 +196,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D>::PER_SM) attend_kernel(Atten
   if (scan[tid] * cols <= pos && pos < scan[tid + 1] * cols) {
     int base = scan[tid] * cols, b = tid * run, kl;
     for (;; ++b) {
-      const int n = tiles_of<KT>(p, b, kl).y * cols;
+      const int n = tiles_of(p, b, kl).y * cols;
       if (pos < base + n) break;
       base += n;
     }
@@ -194,7 +205,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D>::PER_SM) attend_kernel(Atten
   // sequences without visible keys: their rows are 0
   for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
     int kl;
-    if (tiles_of<KT>(p, b, kl).y > 0) continue;
+    if (tiles_of(p, b, kl).y > 0) continue;
     uint32_t* o = reinterpret_cast<uint32_t*>(p.o + (int64_t)b * p.L * p.H * D);
     for (int64_t i = tid; i < (int64_t)p.L * p.H * D / 2; i += THREADS) o[i] = 0;
   }
@@ -202,12 +213,21 @@ __global__ void __launch_bounds__(THREADS, Shape<D>::PER_SM) attend_kernel(Atten
   if (pos >= end) return;
   __syncthreads();
   int b = start_b, base = start_base;
-  const uint32_t slot0 = smem_u32(ring) + warp * (STAGES * S::TILE);
+  unsigned char* slots = ring + warp * (STAGES * S::TILE);  // this warp's tiles: 32 keys, then 32 values
+  // bytes of this lane in a tile: TMA stores the 16-byte chunk q of row r at q ^ (r & 7) (rows of 128
+  // bytes) or q ^ ((r >> 1) & 3) (64 bytes), which spreads the rows that a load touches over the banks
+  uint32_t koff[HALVES], voff[2];
+#pragma unroll
+  for (int h = 0; h < HALVES; ++h) koff[h] = g * D + (((h * 4 + c) ^ (D == 128 ? g : g >> 1)) << 4);
+#pragma unroll
+  for (int y = 0; y < 2; ++y)
+    voff[y] = KT * D + (2 * c + y) * D + (D == 128 ? (g ^ (2 * c + y)) << 4 : (((g >> 1) ^ c) << 4) + (g & 1) * 8);
+  uint32_t issued = 0, used = 0;  // tiles of this warp, over all its pieces
   const float ninf = -INFINITY;
 
   while (pos < end) {
     int kv_len;
-    const int2 tl = tiles_of<KT>(p, b, kv_len);
+    const int2 tl = tiles_of(p, b, kv_len);
     const int nt = tl.y;
     if (pos >= base + nt * cols) {
       base += nt * cols;
@@ -220,68 +240,47 @@ __global__ void __launch_bounds__(THREADS, Shape<D>::PER_SM) attend_kernel(Atten
     const int hk = col / p.RT, rt = col - hk * p.RT;
     const int rows = min(ROWS, rows_all - rt * ROWS);
     const int64_t bh = (int64_t)b * p.Hkv + hk;
-    const uint8_t* kb = p.k + bh * p.cap * D;
-    const uint8_t* vb = p.v + bh * p.cap * D;
     const uint8_t* ksb = p.ks + bh * p.nblk;
     const uint8_t* vsb = p.vs + bh * p.nblk;
     const int my_n = (n - warp + WARPS - 1) / WARPS;                  // tiles of this warp: warp, warp + 4, ...
     const int key_first = (tl.x + ta + warp) * KT;
 
-    auto load_tile = [&](int i) {
-      const int key0 = key_first + i * (WARPS * KT);
-      const uint32_t dst = slot0 + (i % STAGES) * S::TILE;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int key = key0 + u * 16 + j * 8 + g;
-          const bool ok = key < kv_len;
-          const uint8_t* src = kb + (int64_t)(ok ? key : 0) * D + c * 16;
-#pragma unroll
-          for (int h = 0; h < HALVES; ++h)
-            cp16(dst + (u * 2 * HALVES + j * HALVES + h) * 512 + lane * 16, src + h * 64, ok);
-        }
-        const uint32_t vdst = dst + KT * D + u * 16 * D;
-#pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) {
-          const int key = key0 + u * 16 + (i4 >> 1) * 8 + 2 * c + (i4 & 1);
-          const bool ok = key < kv_len;
-          const uint8_t* src = vb + (int64_t)(ok ? key : 0) * D + g * VB;
-          if constexpr (D == 128) cp16(vdst + i4 * 512 + lane * 16, src, ok);
-          else cp_async_8(vdst + i4 * 256 + lane * 8, src, ok);
-        }
+    auto load_tile = [&](int i) {  // into the slot that the warp has finished reading
+      const uint32_t st = issued++ % STAGES;
+      if (lane == 0) {
+        const int key0 = key_first + i * (WARPS * KT);
+        mbar_arrive_expect_tx(&full[warp][st], S::TILE);
+        tma_load_3d(slots + st * S::TILE, &tmk, &full[warp][st], 0, key0, (int)bh);
+        tma_load_3d(slots + st * S::TILE + KT * D, &tmv, &full[warp][st], 0, key0, (int)bh);
       }
     };
-    // scale bytes of a tile's keys: one a 16-key group, or one a key of this lane
-    constexpr int NS = UNI ? U : 4 * U;
+    // scale bytes of a tile's keys: one a 16-key group, or those of this lane's keys g and g + 8
+    constexpr int NS = UNI ? U : 2 * U;
     int kbyte[NS], vbyte[NS];
-    auto load_scales = [&](int i, int (&kx)[NS], int (&vx)[NS]) {
+    auto load_scales = [&](int i) {
       const int key0 = key_first + i * (WARPS * KT);
 #pragma unroll
-      for (int s = 0; s < NS; ++s) {
-        const int key = UNI ? key0 + s * 16 : key0 + (s >> 2) * 16 + ((s >> 1) & 1) * 8 + 2 * c + (s & 1);
+      for (int x = 0; x < NS; ++x) {
+        const int key = UNI ? key0 + x * 16 : key0 + x * 8 + g;
         const bool ok = key < kv_len;
-        kx[s] = ok ? ksb[key >> p.shift] : kMinScale;
-        vx[s] = ok ? vsb[key >> p.shift] : kMinScale;
+        kbyte[x] = ok ? ksb[key >> p.shift] : kMinScale;
+        vbyte[x] = ok ? vsb[key >> p.shift] : kMinScale;
       }
     };
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) {
+    for (int i = 0; i < STAGES; ++i)
       if (i < my_n) load_tile(i);
-      cp_commit();
-    }
-    if (my_n > 0) load_scales(0, kbyte, vbyte);
+    if (my_n > 0) load_scales(0);
 
-    // ---- query rows g and g + 8 of the tile, scaled to f16
-    uint32_t qa[D / 16][4];
-    float rowf[2];
-    int qpos[2];
+    // ---- the queries, scaled to f16: row 8 nt + g of the tile is column g of the nt-th B operand
+    uint32_t qb[NT][D / 16][2];
+    float rowf[NT][2];  // of the rows 8 nt + 2c, 2c + 1, which this lane's scores belong to
+    int qpos[NT][2];
 #pragma unroll
-    for (int r2 = 0; r2 < 2; ++r2) {
-      const int r = rt * ROWS + g + r2 * 8;
+    for (int nt8 = 0; nt8 < NT; ++nt8) {
+      const int r = rt * ROWS + nt8 * 8 + g;
       const bool ok = r < rows_all;
       const int gh = ok ? r / p.L : 0, i = ok ? r % p.L : 0;
-      qpos[r2] = kv_len - p.L + i;
       const bf16* src = p.q + b * p.q_sb + i * p.q_st + (int64_t)(hk * G + gh) * p.q_sh + c * 16;
       uint4 w[HALVES * 2];
       uint32_t am = 0;
@@ -298,7 +297,7 @@ __global__ void __launch_bounds__(THREADS, Shape<D>::PER_SM) attend_kernel(Atten
       // 2^(14 - (e - 127)); rows with an infinity or NaN keep their values (and give NaN)
       const int field = e == 255 ? 127 : min(253, 268 - e);
       const float mul = __int_as_float(field << 23) * p.sign;
-      rowf[r2] = __int_as_float((254 - field) << 23) * p.scale_log2;
+      const float back = __int_as_float((254 - field) << 23) * p.scale_log2;
 #pragma unroll
       for (int h = 0; h < HALVES * 2; ++h) {
         const uint32_t ww[4] = {w[h].x, w[h].y, w[h].z, w[h].w};
@@ -306,148 +305,212 @@ __global__ void __launch_bounds__(THREADS, Shape<D>::PER_SM) attend_kernel(Atten
         for (int k = 0; k < 4; ++k) {
           const float x = __uint_as_float(ww[k] << 16) * mul, y = __uint_as_float(ww[k] & 0xffff0000u) * mul;
           // elements (2k, 2k + 1) of 8: MMA step (k >> 1), its lower or upper k half
-          qa[h * 2 + (k >> 1)][(k & 1) * 2 + r2] = pack_f16(x, y);
+          qb[nt8][h * 2 + (k >> 1)][k & 1] = pack_f16(x, y);
         }
+      }
+#pragma unroll
+      for (int q2 = 0; q2 < 2; ++q2) {
+        rowf[nt8][q2] = __shfl_sync(0xffffffffu, back, (2 * c + q2) * 4);
+        qpos[nt8][q2] = kv_len - p.L + (rt * ROWS + nt8 * 8 + 2 * c + q2) % p.L;
       }
     }
 
-    float m[2] = {ninf, ninf}, l[2] = {0.f, 0.f};
-    float o[VB][4];
+    // m is the maximum less 8 that the sums stand for; `limit` is how far above m a weight may rise
+    // (everything, before the first)
+    float m[NT][2], l[NT][2], limit[NT][2];
+    float o[NT][MT][4];
 #pragma unroll
-    for (int t = 0; t < VB; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+    for (int nt8 = 0; nt8 < NT; ++nt8) {
+      m[nt8][0] = m[nt8][1] = l[nt8][0] = l[nt8][1] = 0.f;
+      limit[nt8][0] = limit[nt8][1] = ninf;
+#pragma unroll
+      for (int t = 0; t < MT; ++t) o[nt8][t][0] = o[nt8][t][1] = o[nt8][t][2] = o[nt8][t][3] = 0.f;
+    }
 
     for (int i = 0; i < my_n; ++i) {
-      if (i + STAGES - 1 < my_n) load_tile(i + STAGES - 1);
-      cp_commit();
       int kx[NS], vx[NS];
 #pragma unroll
-      for (int s = 0; s < NS; ++s) kx[s] = kbyte[s], vx[s] = vbyte[s];
-      if (i + 1 < my_n) load_scales(i + 1, kbyte, vbyte);
-      cp_wait<STAGES - 1>();  // tile i has landed (a lane reads only what it copied itself)
-      const unsigned char* buf = ring + warp * (STAGES * S::TILE) + (i % STAGES) * S::TILE;
+      for (int x = 0; x < NS; ++x) kx[x] = kbyte[x], vx[x] = vbyte[x];
+      if (i + 1 < my_n) load_scales(i + 1);
+      const uint32_t st = used % STAGES;
+      tile_wait(&full[warp][st], (used / STAGES) & 1, p.status);
+      ++used;
+      const unsigned char* buf = slots + st * S::TILE;
       const int key0 = key_first + i * (WARPS * KT);
-      // ---- S = Q K^T
-      float s[2 * U][4];
+      // ---- S^T = K Q^T (16 keys x 8 queries an MMA); s[.][u][e]: key 16 u + g + 8 (e >> 1), query 2c + (e & 1)
+      float s[NT][U][4];
 #pragma unroll
-      for (int j = 0; j < 2 * U; ++j) {
-        s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+      for (int u = 0; u < U; ++u) {
+        float s2[NT][4];  // a second chain of accumulations
+#pragma unroll
+        for (int nt8 = 0; nt8 < NT; ++nt8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt8][u][e] = s2[nt8][e] = 0.f;
 #pragma unroll
         for (int h = 0; h < HALVES; ++h) {
-          const uint4 w = *reinterpret_cast<const uint4*>(buf + (j * HALVES + h) * 512 + lane * 16);
-          const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+          const uint4 w0 = *reinterpret_cast<const uint4*>(buf + koff[h] + u * 16 * D);
+          const uint4 w1 = *reinterpret_cast<const uint4*>(buf + koff[h] + (u * 16 + 8) * D);
+          const uint32_t x0[4] = {w0.x, w0.y, w0.z, w0.w}, x1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            uint32_t b0, b1;
-            widen4<INT8>(ww[k], b0, b1);
-            mma_f16(s[j], qa[h * 4 + k], b0, b1);
+            uint32_t a[4];
+            widen4<INT8>(x0[k], a[0], a[2]);
+            widen4<INT8>(x1[k], a[1], a[3]);
+#pragma unroll
+            for (int nt8 = 0; nt8 < NT; ++nt8)
+              mma_f16(k & 1 ? s2[nt8] : s[nt8][u], a, qb[nt8][h * 4 + k][0], qb[nt8][h * 4 + k][1]);
           }
         }
+#pragma unroll
+        for (int nt8 = 0; nt8 < NT; ++nt8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt8][u][e] += s2[nt8][e];
       }
-      // ---- t = s * f + log2 s_v, masked
-      float lv[NS], isv[NS];
+      // ---- t = s * f + log2 s_v - m, masked
+      float isv[NS];
 #pragma unroll
       for (int x = 0; x < NS; ++x) {
-        lv[x] = vx[x] == kBadScale ? __int_as_float(0x7fffffff) : (float)(vx[x] - 127);
-        isv[x] = scale_inverse(min(vx[x], 253));
-      }
-      float f[2][NS];
-#pragma unroll
-      for (int x = 0; x < NS; ++x) {
+        const float lv = vx[x] == kBadScale ? __int_as_float(0x7fffffff) : (float)(vx[x] - 127);
         const float sk = scale_value(kx[x]);
-        f[0][x] = rowf[0] * sk, f[1][x] = rowf[1] * sk;
+        isv[x] = scale_inverse(min(vx[x], 253));
+#pragma unroll
+        for (int nt8 = 0; nt8 < NT; ++nt8)
+#pragma unroll
+          for (int q2 = 0; q2 < 2; ++q2) {
+            const float f = rowf[nt8][q2] * sk, add = lv - m[nt8][q2];
+            if constexpr (UNI) {
+              s[nt8][x][q2] = fmaf(s[nt8][x][q2], f, add);
+              s[nt8][x][2 + q2] = fmaf(s[nt8][x][2 + q2], f, add);
+            } else {
+              float& t = s[nt8][x >> 1][2 * (x & 1) + q2];
+              t = fmaf(t, f, add);
+            }
+          }
       }
       // every row sees the whole tile
       const bool inner = key0 + KT <= kv_len && (p.right < 0 || key0 + KT - 1 <= kv_len - p.L + p.right) &&
                          (p.left < 0 || key0 >= kv_len - 1 - p.left);
-      float mx[2] = {ninf, ninf};
+      if (!inner) {
 #pragma unroll
-      for (int j = 0; j < 2 * U; ++j)
+        for (int nt8 = 0; nt8 < NT; ++nt8)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r2 = e >> 1, x = UNI ? j >> 1 : j * 2 + (e & 1);
-          s[j][e] = fmaf(s[j][e], f[r2][x], lv[x]);
-          if (!inner) {
-            const int key = key0 + j * 8 + 2 * c + (e & 1);
-            const bool vis = key < kv_len && (p.right < 0 || key <= qpos[r2] + p.right) &&
-                             (p.left < 0 || key >= qpos[r2] - p.left);
-            if (!vis) s[j][e] = ninf;
-          }
-          mx[r2] = fmaxf(mx[r2], s[j][e]);
-        }
-      // ---- follow the maximum; O is rescaled rarely
-      if (__any_sync(0xffffffffu, mx[0] > m[0] + 15.f || mx[1] > m[1] + 15.f)) {
+          for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int r2 = 0; r2 < 2; ++r2) {
-          float x = mx[r2];
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-          const float to = x > m[r2] + 15.f ? x - 8.f : m[r2];
-          const float corr = to == m[r2] ? 1.f : ex2(m[r2] - to);
-          m[r2] = to;
-          l[r2] *= corr;
-#pragma unroll
-          for (int t = 0; t < VB; ++t) o[t][2 * r2] *= corr, o[t][2 * r2 + 1] *= corr;
-        }
+            for (int e = 0; e < 4; ++e) {
+              const int key = key0 + u * 16 + (e >> 1) * 8 + g, at = qpos[nt8][e & 1];
+              const bool vis = key < kv_len && (p.right < 0 || key <= at + p.right) && (p.left < 0 || key >= at - p.left);
+              if (!vis) s[nt8][u][e] = ninf;
+            }
       }
-      const float mu[2] = {m[0] == ninf ? 0.f : m[0], m[1] == ninf ? 0.f : m[1]};
+      // ---- follow the maximum; O is rescaled rarely
+      bool rise = false;
 #pragma unroll
-      for (int j = 0; j < 2 * U; ++j)
+      for (int nt8 = 0; nt8 < NT; ++nt8)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r2 = e >> 1, x = UNI ? j >> 1 : j * 2 + (e & 1);
-          s[j][e] = ex2(s[j][e] - mu[r2]);
-          l[r2] = fmaf(s[j][e], isv[x], l[r2]);
+        for (int q2 = 0; q2 < 2; ++q2) {
+          float x = ninf;
+#pragma unroll
+          for (int u = 0; u < U; ++u) x = fmax3(x, s[nt8][u][q2], s[nt8][u][2 + q2]);
+          rise |= x > limit[nt8][q2];
         }
-      // ---- O += P V
+      if (__any_sync(0xffffffffu, rise)) {
+#pragma unroll
+        for (int nt8 = 0; nt8 < NT; ++nt8)
+#pragma unroll
+          for (int q2 = 0; q2 < 2; ++q2) {
+            float x = ninf;
+#pragma unroll
+            for (int u = 0; u < U; ++u) x = fmax3(x, s[nt8][u][q2], s[nt8][u][2 + q2]);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+            if (x > limit[nt8][q2]) {
+              // nothing is summed before the first
+              const float up = x - 8.f, corr = limit[nt8][q2] == ninf ? 0.f : ex2(-up);
+              limit[nt8][q2] = 15.f;
+              m[nt8][q2] += up;
+              l[nt8][q2] *= corr;
+#pragma unroll
+              for (int t = 0; t < MT; ++t) o[nt8][t][q2] *= corr, o[nt8][t][2 + q2] *= corr;
+#pragma unroll
+              for (int u = 0; u < U; ++u) s[nt8][u][q2] -= up, s[nt8][u][2 + q2] -= up;
+            }
+          }
+      }
+      // ---- weights and their sums; P^T as the B operand of O^T += V^T P^T
+      uint32_t pb[NT][U][2];
+#pragma unroll
+      for (int nt8 = 0; nt8 < NT; ++nt8)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          float (&w)[4] = s[nt8][u];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = ex2(w[e]);
+#pragma unroll
+          for (int q2 = 0; q2 < 2; ++q2) {
+            if constexpr (UNI) {
+              l[nt8][q2] = fmaf(w[q2] + w[2 + q2], isv[u], l[nt8][q2]);
+            } else {
+              l[nt8][q2] = fmaf(w[q2], isv[2 * u], l[nt8][q2]);
+              l[nt8][q2] = fmaf(w[2 + q2], isv[2 * u + 1], l[nt8][q2]);
+            }
+          }
+          pb[nt8][u][0] = transpose8(pack_f16(w[0], w[1]));
+          pb[nt8][u][1] = transpose8(pack_f16(w[2], w[3]));
+        }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const uint32_t pa[4] = {pack_f16(s[2 * u][0], s[2 * u][1]), pack_f16(s[2 * u][2], s[2 * u][3]),
-                                pack_f16(s[2 * u + 1][0], s[2 * u + 1][1]),
-                                pack_f16(s[2 * u + 1][2], s[2 * u + 1][3])};
-        uint32_t vw[4][VB / 4];
-        const unsigned char* vbuf = buf + KT * D + u * 16 * D;
+        uint32_t vw[4][VB / 4];  // keys 2c, 2c + 1, 2c + 8, 2c + 9; head dims g * VB ..
 #pragma unroll
         for (int i4 = 0; i4 < 4; ++i4) {
+          const unsigned char* src = buf + voff[i4 & 1] + (u * 16 + (i4 >> 1) * 8) * D;
           if constexpr (D == 128) {
-            const uint4 w = *reinterpret_cast<const uint4*>(vbuf + i4 * 512 + lane * 16);
+            const uint4 w = *reinterpret_cast<const uint4*>(src);
             vw[i4][0] = w.x, vw[i4][1] = w.y, vw[i4][2] = w.z, vw[i4][3] = w.w;
           } else {
-            const uint2 w = *reinterpret_cast<const uint2*>(vbuf + i4 * 256 + lane * 8);
+            const uint2 w = *reinterpret_cast<const uint2*>(src);
             vw[i4][0] = w.x, vw[i4][1] = w.y;
           }
         }
+        if (!inner) {  // past the length there may be any bytes, NaN among them
+#pragma unroll
+          for (int i4 = 0; i4 < 4; ++i4)
+            if (key0 + u * 16 + (i4 >> 1) * 8 + 2 * c + (i4 & 1) >= kv_len)
+#pragma unroll
+              for (int x = 0; x < VB / 4; ++x) vw[i4][x] = 0;
+        }
 #pragma unroll
         for (int x = 0; x < VB / 4; ++x) {
-          uint32_t b0[4], b1[4];  // f16 pairs of keys (2c, 2c + 1) and (2c + 8, 2c + 9) for columns 4x .. 4x + 3
-          widen4<INT8>(__byte_perm(vw[0][x], vw[1][x], 0x5140), b0[0], b0[1]);
-          widen4<INT8>(__byte_perm(vw[0][x], vw[1][x], 0x7362), b0[2], b0[3]);
-          widen4<INT8>(__byte_perm(vw[2][x], vw[3][x], 0x5140), b1[0], b1[1]);
-          widen4<INT8>(__byte_perm(vw[2][x], vw[3][x], 0x7362), b1[2], b1[3]);
+          // MMA tile t = 2x + k: its rows g and g + 8 are the head dims g * VB + 2t and + 1
+          uint32_t a[2][4];
+          widen4<INT8>(__byte_perm(vw[0][x], vw[1][x], 0x5140), a[0][0], a[0][1]);
+          widen4<INT8>(__byte_perm(vw[2][x], vw[3][x], 0x5140), a[0][2], a[0][3]);
+          widen4<INT8>(__byte_perm(vw[0][x], vw[1][x], 0x7362), a[1][0], a[1][1]);
+          widen4<INT8>(__byte_perm(vw[2][x], vw[3][x], 0x7362), a[1][2], a[1][3]);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) mma_f16(o[4 * x + k], pa, b0[k], b1[k]);
+          for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int nt8 = 0; nt8 < NT; ++nt8) mma_f16(o[nt8][2 * x + k], a[k], pb[nt8][u][0], pb[nt8][u][1]);
         }
       }
+      __syncwarp();
+      if (i + STAGES < my_n) load_tile(i + STAGES);
     }
-    cp_wait<0>();
-#pragma unroll
-    for (int r2 = 0; r2 < 2; ++r2) {
-      l[r2] += __shfl_xor_sync(0xffffffffu, l[r2], 1);
-      l[r2] += __shfl_xor_sync(0xffffffffu, l[r2], 2);
-    }
-    // ---- join the warps through shared memory.  o[t][.] holds columns n = 2c, 2c + 1 of MMA tile t,
-    // which are head dims n * VB + t; kept as [row][t][n] until the end.
+    // ---- join the warps through shared memory
     __syncthreads();
     float* ow = reinterpret_cast<float*>(ring);
-    if (c == 0) {
-      wM[warp][g] = m[0], wM[warp][g + 8] = m[1];
-      wL[warp][g] = l[0], wL[warp][g + 8] = l[1];
-    }
 #pragma unroll
-    for (int t = 0; t < VB; ++t) {
-      float* dst = ow + (warp * ROWS + g) * S::OROW + t * 8 + 2 * c;
-      *reinterpret_cast<float2*>(dst) = make_float2(o[t][0], o[t][1]);
-      *reinterpret_cast<float2*>(dst + 8 * S::OROW) = make_float2(o[t][2], o[t][3]);
-    }
+    for (int nt8 = 0; nt8 < NT; ++nt8)
+#pragma unroll
+      for (int q2 = 0; q2 < 2; ++q2) {
+        const int r = nt8 * 8 + 2 * c + q2;
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[nt8][q2] += __shfl_xor_sync(0xffffffffu, l[nt8][q2], d);
+        if (g == 0) wM[warp][r] = limit[nt8][q2] == ninf ? ninf : m[nt8][q2], wL[warp][r] = l[nt8][q2];
+        float4* dst = reinterpret_cast<float4*>(ow + (warp * ROWS + r) * S::OROW + g * VB);
+#pragma unroll
+        for (int t = 0; t < MT; t += 2)
+          dst[t / 2] = make_float4(o[nt8][t][q2], o[nt8][t][2 + q2], o[nt8][t + 1][q2], o[nt8][t + 1][2 + q2]);
+      }
     __syncthreads();
     const bool whole = ta == 0 && n == nt;
     const int64_t slot = (int64_t)blockIdx.x * 2 + (pos != run_first);
@@ -466,39 +529,40 @@ __global__ void __launch_bounds__(THREADS, Shape<D>::PER_SM) attend_kernel(Atten
       if (!whole && tid < rows) *reinterpret_cast<float2*>(p.ml + (slot * ROWS + tid) * 2) = make_float2(M, L);
     }
     __syncthreads();
-    for (int e = tid; e < rows * VB; e += THREADS) {  // (row, t): n = 0 .. 7
-      const int r = e / VB, t = e % VB;
+    for (int e = tid; e < rows * VB; e += THREADS) {  // 8 head dims of a row
+      const int r = e / VB, d = (e % VB) * 8;
       float x[8] = {};
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
         const float f = wM[w][r];
         if (f == 0.f) continue;
-        const float4* src = reinterpret_cast<const float4*>(ow + (w * ROWS + r) * S::OROW + t * 8);
+        const float4* src = reinterpret_cast<const float4*>(ow + (w * ROWS + r) * S::OROW + d);
         const float4 u = src[0], v = src[1];
         x[0] += f * u.x, x[1] += f * u.y, x[2] += f * u.z, x[3] += f * u.w;
         x[4] += f * v.x, x[5] += f * v.y, x[6] += f * v.z, x[7] += f * v.w;
       }
       if (whole) {
-        bf16* o = out_row(p, b, hk, rt * ROWS + r, D) + t;
         const float inv = rL[r] == 0.f ? 0.f : 1.f / rL[r];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) o[k * VB] = __float2bfloat16(x[k] * inv);
+        *reinterpret_cast<uint4*>(out_row(p, b, hk, rt * ROWS + r, D) + d) =
+            make_uint4(pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv),
+                       pack_bf16x2(x[4] * inv, x[5] * inv), pack_bf16x2(x[6] * inv, x[7] * inv));
       } else {
-        float4* dst = reinterpret_cast<float4*>(p.part + (slot * ROWS + r) * D + t * 8);
+        float4* dst = reinterpret_cast<float4*>(p.part + (slot * ROWS + r) * D + d);
         dst[0] = make_float4(x[0], x[1], x[2], x[3]);
         dst[1] = make_float4(x[4], x[5], x[6], x[7]);
       }
     }
-    __syncthreads();  // the merge buffer is the ring
+    fence_proxy_async_smem();  // the merge buffer is the ring, which TMA writes next
+    __syncthreads();
     pos += n;
   }
 }
 
 // Joins the partials of the columns that several CTAs share, in the order of the CTAs; one CTA a
 // column.  Launched so that everything up to the wait overlaps attend_kernel.
-template <int D>
+template <int D, int NT>
 __global__ void __launch_bounds__(THREADS) join_kernel(AttendParams p) {
-  constexpr int KT = Shape<D>::KT, VB = D / 8, D4 = D / 4, MAXE = ROWS * D4 / THREADS;
+  constexpr int ROWS = 8 * NT, D4 = D / 4, MAXE = ROWS * D4 / THREADS, PER = THREADS / ROWS;
   extern __shared__ float wt[];  // [partials][ROWS] weights
   __shared__ int red[WARPS];
   __shared__ float sL[ROWS];
@@ -508,12 +572,12 @@ __global__ void __launch_bounds__(THREADS) join_kernel(AttendParams p) {
   const int b = blockIdx.x / cols, col = blockIdx.x - b * cols;
   int kl, all = 0, before = 0;
   for (int i = tid; i < p.B; i += THREADS) {
-    const int n = tiles_of<KT>(p, i, kl).y;
+    const int n = tiles_of(p, i, kl).y;
     all += n;
     if (i < b) before += n;
   }
   const Runs runs(block_sum(all, red) * cols, p.grid);
-  const int nt = tiles_of<KT>(p, b, kl).y;
+  const int nt = tiles_of(p, b, kl).y;
   const int cf = block_sum(before, red) * cols + col * nt;
   grid_dependency_wait();
   if (nt == 0) return;
@@ -524,23 +588,24 @@ __global__ void __launch_bounds__(THREADS) join_kernel(AttendParams p) {
   // the column is the first piece of every CTA but c0, and of c0 only if c0's run starts with it
   const bool late = runs.first(c0) != cf;
   auto slot = [&](int x) { return ((int64_t)c0 + x) * 2 + (x == 0 && late); };
-  {  // rows' maxima, weights and sums: 8 threads a row
-    const int r = tid >> 3;
+  {  // rows' maxima, weights and sums: PER threads a row
+    const int r = tid / PER, first = tid % PER;
     float M = -INFINITY, L = 0.f;
     if (r < rows)
-      for (int x = tid & 7; x < nc; x += 8) M = fmaxf(M, __ldcg(p.ml + (slot(x) * ROWS + r) * 2));
+#pragma unroll 4
+      for (int x = first; x < nc; x += PER) M = fmaxf(M, p.ml[(slot(x) * ROWS + r) * 2]);
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    for (int o = 1; o < PER; o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     if (r < rows)
-      for (int x = tid & 7; x < nc; x += 8) {
-        const float2 ml = __ldcg(reinterpret_cast<const float2*>(p.ml + (slot(x) * ROWS + r) * 2));
+      for (int x = first; x < nc; x += PER) {
+        const float2 ml = *reinterpret_cast<const float2*>(p.ml + (slot(x) * ROWS + r) * 2);
         const float f = part_weight(ml.x, ml.y, M);
         wt[x * ROWS + r] = f;
         if (f != 0.f) L += f * ml.y;
       }
 #pragma unroll
-    for (int o = 1; o < 8; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-    if ((tid & 7) == 0) sL[r] = L;
+    for (int o = 1; o < PER; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    if (first == 0) sL[r] = L;
   }
   __syncthreads();
   // O as float4 columns; with few rows, groups of threads take every groups-th partial
@@ -552,11 +617,19 @@ __global__ void __launch_bounds__(THREADS) join_kernel(AttendParams p) {
     const int r = e / D4;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
     if (e < n4 && first < groups) {
-#pragma unroll 8
-      for (int x = first; x < nc; x += groups) {
-        const float f = wt[x * ROWS + r];
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part + slot(x) * ROWS * D) + e);
-        if (f != 0.f) a.x += f * v.x, a.y += f * v.y, a.z += f * v.z, a.w += f * v.w;
+      for (int x0 = first; x0 < nc; x0 += 8 * groups) {  // eight loads at a time
+        float4 v[8];
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+          const int x = x0 + y * groups;
+          v[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (x < nc) v[y] = *(reinterpret_cast<const float4*>(p.part + slot(x) * ROWS * D) + e);
+        }
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+          const float f = wt[min(x0 + y * groups, nc - 1) * ROWS + r];  // v is 0 where f does not belong to it
+          a.x += f * v[y].x, a.y += f * v[y].y, a.z += f * v[y].z, a.w += f * v[y].w;
+        }
       }
     }
     if (groups > 1) {
@@ -569,11 +642,9 @@ __global__ void __launch_bounds__(THREADS) join_kernel(AttendParams p) {
         }
     }
     if (groups > 1 ? tid < n4 : e < n4) {
-      const int tn = (e % D4) * 4;
-      bf16* o = out_row(p, b, hk, rt * ROWS + r, D) + (tn & 7) * VB + (tn >> 3);
       const float inv = sL[r] == 0.f ? 0.f : 1.f / sL[r];
-      o[0] = __float2bfloat16(a.x * inv), o[VB] = __float2bfloat16(a.y * inv);
-      o[2 * VB] = __float2bfloat16(a.z * inv), o[3 * VB] = __float2bfloat16(a.w * inv);
+      *reinterpret_cast<uint2*>(out_row(p, b, hk, rt * ROWS + r, D) + (e % D4) * 4) =
+          make_uint2(pack_bf16x2(a.x * inv, a.y * inv), pack_bf16x2(a.z * inv, a.w * inv));
     }
   }
 }
@@ -629,61 +700,69 @@ torch::Tensor kv8_attend(torch::Tensor q, torch::Tensor keys, torch::Tensor valu
   if (!rows16(q)) q = q.clone(at::MemoryFormat::Contiguous);
   AttendParams p{};
   p.q = (const bf16*)q.data_ptr();
-  p.k = c.data[0], p.v = c.data[1], p.ks = c.scale[0], p.vs = c.scale[1];
+  p.ks = c.scale[0], p.vs = c.scale[1];
   p.seqlens = lens;
   p.o = (bf16*)o.data_ptr();
   p.q_sb = q.stride(0), p.q_st = q.stride(1), p.q_sh = q.stride(2);
-  p.B = c.B, p.L = L, p.H = H, p.Hkv = c.Hkv, p.RT = (G * L + ROWS - 1) / ROWS;
+  const int nt = G * L <= 8 ? 1 : 2, rows = 8 * nt;
+  p.B = c.B, p.L = L, p.H = H, p.Hkv = c.Hkv, p.RT = (G * L + rows - 1) / rows;
   p.cap = c.cap, p.nblk = c.nblk, p.shift = c.shift, p.extra = extra;
   p.left = (int)left, p.right = (int)right;
   p.scale_log2 = (float)(std::abs(scale) * 1.4426950408889634), p.sign = scale < 0 ? -1.f : 1.f;
   static int sms[64] = {0};
   if (!sms[c.device]) C10_CUDA_CHECK(cudaDeviceGetAttribute(&sms[c.device], cudaDevAttrMultiProcessorCount, c.device));
-  const int per_sm = c.D == 64 ? Shape<64>::PER_SM : Shape<128>::PER_SM;
-  const int kt = c.D == 64 ? Shape<64>::KT : Shape<128>::KT;
+  const int per_sm = c.D == 64 ? (nt == 1 ? Shape<64, 1>::PER_SM : Shape<64, 2>::PER_SM)
+                               : (nt == 1 ? Shape<128, 1>::PER_SM : Shape<128, 2>::PER_SM);
   int64_t span = c.cap;  // most keys a sequence can show
-  if (left >= 0) span = std::min<int64_t>(span, left + L + kt);
+  if (left >= 0) span = std::min<int64_t>(span, left + L + KT);
   const int64_t columns = (int64_t)c.B * c.Hkv * p.RT;
-  const int64_t want = (columns * ((span + kt - 1) / kt) + WARPS - 1) / WARPS;
+  const int64_t want = (columns * ((span + KT - 1) / KT) + WARPS - 1) / WARPS;
   const int grid = (int)std::min<int64_t>(want, (int64_t)sms[c.device] * per_sm);
-  TORCH_CHECK(columns * ((c.cap + kt - 1) / kt) <= INT32_MAX, who, ": too many sequences x heads x keys");
+  TORCH_CHECK(columns * ((c.cap + KT - 1) / KT) <= INT32_MAX, who, ": too many sequences x heads x keys");
   // workspace: partials of at most two pieces a CTA
-  const int64_t part = (int64_t)grid * 2 * ROWS * c.D, ml = (int64_t)grid * 2 * ROWS * 2;
+  const int64_t part = (int64_t)grid * 2 * rows * c.D, ml = (int64_t)grid * 2 * rows * 2;
   auto work = torch::empty({part + ml}, q.options().dtype(at::kFloat));
   p.part = work.data_ptr<float>();
   p.ml = p.part + part;
   p.grid = grid;
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
-  auto start = [&](auto kern, int blocks, int smem, bool overlap) {
+  auto start = [&](auto kern, int blocks, int smem, bool overlap, auto... args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = blocks, cfg.blockDim = THREADS, cfg.dynamicSmemBytes = smem, cfg.stream = st;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr, cfg.numAttrs = overlap ? 1 : 0;
-    C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, p));
+    C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, args...));
   };
   const bool uni = c.shift >= 4;
+  p.status = device_status();
+  const CUtensorMapSwizzle swizzle = c.D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+  auto map = [&](uint8_t* base) {
+    return make_tmap_3d(base, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, c.D, c.cap, (int64_t)c.B * c.Hkv, c.D,
+                        (int64_t)c.cap * c.D, c.D, KT, swizzle);
+  };
+  const CUtensorMap tmk = map(c.data[0]), tmv = map(c.data[1]);
   auto launch = [&](auto kern, SmemOptIn& attr, int smem) {
     C10_CUDA_CHECK(attr.ensure(kern, smem));
-    start(kern, grid, smem, extra > 0);  // the kernel before it is then append()'s
+    start(kern, grid, smem, extra > 0, tmk, tmv, p);  // the kernel before it is then append()'s
   };
-  static SmemOptIn a[8];
-#define KV8_CASE(d, i8, un) \
-  if (c.D == d && c.int8 == i8 && uni == un) \
-    launch(attend_kernel<d, i8, un>, a[(d == 128) * 4 + i8 * 2 + un], Shape<d>::SMEM)
-  KV8_CASE(64, false, false);
-  KV8_CASE(64, false, true);
-  KV8_CASE(64, true, false);
-  KV8_CASE(64, true, true);
-  KV8_CASE(128, false, false);
-  KV8_CASE(128, false, true);
-  KV8_CASE(128, true, false);
-  KV8_CASE(128, true, true);
+  static SmemOptIn a[16];
+#define KV8_CASE(d, n, i8, un)                                 \
+  if (c.D == d && nt == n && c.int8 == i8 && uni == un)        \
+    launch(attend_kernel<d, n, i8, un>, a[(d == 128) * 8 + (n == 2) * 4 + i8 * 2 + un], Shape<d, n>::SMEM)
+#define KV8_CASES(d, n)       \
+  KV8_CASE(d, n, false, false); \
+  KV8_CASE(d, n, false, true);  \
+  KV8_CASE(d, n, true, false);  \
+  KV8_CASE(d, n, true, true);   \
+  if (c.D == d && nt == n) start(join_kernel<d, n>, (int)columns, grid * rows * (int)sizeof(float), true, p)
+  KV8_CASES(64, 1);
+  KV8_CASES(64, 2);
+  KV8_CASES(128, 1);
+  KV8_CASES(128, 2);
+#undef KV8_CASES
 #undef KV8_CASE
-  const int weights = grid * ROWS * (int)sizeof(float);
-  if (c.D == 64) start(join_kernel<64>, (int)columns, weights, true);
-  else start(join_kernel<128>, (int)columns, weights, true);
   return o;
 }
 
