@@ -13,14 +13,15 @@
 //
 // A decode step reads every visible byte of the cache once and does little with it, so it is
 // bound by HBM.  One work list holds the 16-key-multiple tiles of all (sequence, KV head,
-// 16-row tile) columns; every CTA takes an equal run of it, computed on the device from the
-// lengths (ragged batches stay balanced, a captured CUDA graph stays valid).  The four warps
-// of a CTA take its tiles in turn, each through a ring of its own that TMA fills (32 keys and 32
-// values, two bulk copies), so they never wait for one another inside a column.  Keys are the M
+// row tile) columns; every warp takes an equal run of it, computed on the device from the
+// lengths (ragged batches stay balanced, a captured CUDA graph stays valid).  Every warp has a run
+// of its own, which it reads through a ring of its own that TMA fills (32 keys and 32 values a
+// tile, two bulk copies), running ahead over the ends of columns; warps never wait for one
+// another.  Keys are the M
 // side of Q K^T and head dims that of P V, so that one 8-column tile holds up to 8 query rows;
 // the contraction index of the first and the row index of the second are permuted to make a
 // lane's bytes contiguous in shared memory.
-// A column that one CTA covers is written at once; else the CTAs leave fp32 partials and a
+// A column that one warp covers is written at once; else the warps leave fp32 partials and a
 // second kernel, whose start overlaps the first, joins them in order: no atomics, and results
 // that do not depend on timing.
 #include <torch/extension.h>
@@ -40,6 +41,7 @@ namespace kv8 {
 constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
 constexpr int KT = 32;        // keys of a tile
+constexpr int JOIN_CHUNK = 32;  // partials that join_kernel copies at a time
 
 struct AttendParams {
   const bf16* q;       // (B, L, H, D)
@@ -47,9 +49,9 @@ struct AttendParams {
   const uint8_t* vs;
   const int* seqlens;  // (B)
   bf16* o;             // (B, L, H, D) contiguous
-  float* part;         // [grid][2][rows][D] partial O of a CTA's first and last piece
-  float* ml;           // [grid][2][rows][2] their maxima and sums
-  int grid;            // CTAs of attend_kernel
+  float* part;         // [warps][2][rows][D] partial O of a warp's first and last piece
+  float* ml;           // [warps][2][rows][2] their maxima and sums
+  int warps;           // of attend_kernel
   int* status;
   int64_t q_sb, q_st, q_sh;
   int B, L, H, Hkv, RT, cap, nblk, shift;
@@ -103,9 +105,7 @@ struct Shape {
   static constexpr int STAGES = D == 64 ? 3 : 1 + NT;
   static constexpr int PER_SM = (D == 64 ? 4 : 3) - (NT - 1);
   static constexpr int TILE = KT * D * 2;  // bytes of a tile's keys and values
-  static constexpr int RING = WARPS * STAGES * TILE;
-  static constexpr int OROW = D + 4;       // floats of a row in the merge buffer
-  static constexpr int SMEM = RING > WARPS * ROWS * OROW * 4 ? RING : WARPS * ROWS * OROW * 4;
+  static constexpr int SMEM = WARPS * STAGES * TILE;
 };
 // Tiles of a sequence that some query sees: [t0, t0 + n).
 __device__ __forceinline__ int2 tiles_of(const AttendParams& p, int b, int& kv_len) {
@@ -116,19 +116,35 @@ __device__ __forceinline__ int2 tiles_of(const AttendParams& p, int b, int& kv_l
   return make_int2(t0, (kv_len + KT - 1) / KT - t0);
 }
 
-// The work list: `total` tiles in runs of `per` or, for the first `rem` CTAs, per + 1.
+// The work list: `total` tiles in runs of `per` or, for the first `rem` warps, per + 1.
 struct Runs {
   int total, active, per, rem;
-  __device__ __forceinline__ Runs(int total_, int grid) {
+  __device__ __forceinline__ Runs(int total_, int warps) {
     total = total_;
-    // as many CTAs take part as get at least one tile a warp
-    active = max(1, min(grid, (total + WARPS - 1) / WARPS));
-    per = total / active, rem = total - per * active;
+    active = min(warps, total);  // 0 where nothing is visible: no warp has a run
+    per = total / max(active, 1), rem = total - per * active;
   }
-  __device__ __forceinline__ int first(int cta) const { return cta * per + min(cta, rem); }
+  __device__ __forceinline__ int first(int w) const { return w * per + min(w, rem); }
   __device__ __forceinline__ int owner(int at) const {
     const int cut = rem * (per + 1);
     return at < cut ? at / (per + 1) : rem + (at - cut) / per;
+  }
+};
+
+// Walks the tiles of the list: sequence b, column col (KV head and row tile), tile t of its nt.
+struct Walk {
+  int b, col, t, nt, t0, kv_len;
+  __device__ __forceinline__ void enter(const AttendParams& p, int b_) {
+    b = b_;
+    const int2 tl = tiles_of(p, b, kv_len);
+    t0 = tl.x, nt = tl.y;
+  }
+  __device__ __forceinline__ void next_column(const AttendParams& p, int cols) {
+    t = 0;
+    if (++col < cols) return;
+    col = 0;
+    do enter(p, b + 1);
+    while (nt == 0 && b < p.B - 1);
   }
 };
 
@@ -158,8 +174,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ C
   extern __shared__ __align__(1024) unsigned char ring[];
   __shared__ uint64_t full[WARPS][STAGES];
   __shared__ int scan[THREADS + 1];
-  __shared__ int start_base, start_b;
-  __shared__ float wM[WARPS][ROWS], wL[WARPS][ROWS], rL[ROWS];
+  __shared__ int2 start[WARPS];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int G = p.H / p.Hkv, rows_all = G * p.L;
   const int cols = p.Hkv * p.RT;  // columns a sequence
@@ -190,17 +205,21 @@ attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ C
     if (tid == 0) scan[0] = 0;
     __syncthreads();
   }
-  const Runs runs(scan[THREADS] * cols, gridDim.x);
-  int pos = runs.first(blockIdx.x);
-  const int run_first = pos, end = blockIdx.x < runs.active ? runs.first(blockIdx.x + 1) : pos;
-  if (scan[tid] * cols <= pos && pos < scan[tid + 1] * cols) {
-    int base = scan[tid] * cols, b = tid * run, kl;
-    for (;; ++b) {
-      const int n = tiles_of(p, b, kl).y * cols;
-      if (pos < base + n) break;
-      base += n;
+  const Runs runs(scan[THREADS] * cols, p.warps);
+  // the first runs go to different CTAs, so that short lists spread over the SMs
+  const int me = warp * gridDim.x + blockIdx.x;
+#pragma unroll
+  for (int w = 0; w < WARPS; ++w) {
+    const int at = runs.first(w * gridDim.x + blockIdx.x);
+    if (scan[tid] * cols <= at && at < scan[tid + 1] * cols) {
+      int base = scan[tid] * cols, b = tid * run, kl;
+      for (;; ++b) {
+        const int n = tiles_of(p, b, kl).y * cols;
+        if (at < base + n) break;
+        base += n;
+      }
+      start[w] = make_int2(b, at - base);
     }
-    start_b = b, start_base = base;
   }
   // sequences without visible keys: their rows are 0
   for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
@@ -210,9 +229,14 @@ attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ C
     for (int64_t i = tid; i < (int64_t)p.L * p.H * D / 2; i += THREADS) o[i] = 0;
   }
   grid_dependency_wait();  // the new tokens are in the cache
-  if (pos >= end) return;
   __syncthreads();
-  int b = start_b, base = start_base;
+  if (me >= runs.active) return;
+  int left = runs.first(me + 1) - runs.first(me);  // tiles still to use
+  Walk use;
+  use.enter(p, start[warp].x);
+  use.col = start[warp].y / use.nt, use.t = start[warp].y - use.col * use.nt;
+  Walk get = use;  // runs ahead of `use`, over column ends
+  int to_get = left;
   unsigned char* slots = ring + warp * (STAGES * S::TILE);  // this warp's tiles: 32 keys, then 32 values
   // bytes of this lane in a tile: TMA stores the 16-byte chunk q of row r at q ^ (r & 7) (rows of 128
   // bytes) or q ^ ((r >> 1) & 3) (64 bytes), which spreads the rows that a load touches over the banks
@@ -222,43 +246,37 @@ attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ C
 #pragma unroll
   for (int y = 0; y < 2; ++y)
     voff[y] = KT * D + (2 * c + y) * D + (D == 128 ? (g ^ (2 * c + y)) << 4 : (((g >> 1) ^ c) << 4) + (g & 1) * 8);
-  uint32_t issued = 0, used = 0;  // tiles of this warp, over all its pieces
-  const float ninf = -INFINITY;
-
-  while (pos < end) {
-    int kv_len;
-    const int2 tl = tiles_of(p, b, kv_len);
-    const int nt = tl.y;
-    if (pos >= base + nt * cols) {
-      base += nt * cols;
-      ++b;
-      continue;
+  uint32_t issued = 0, used = 0;
+  auto load_tile = [&]() {  // the next tile, into the slot that the warp has finished reading
+    if (to_get == 0) return;
+    const uint32_t st = issued++ % STAGES;
+    if (lane == 0) {
+      const int key0 = (get.t0 + get.t) * KT, bh = get.b * p.Hkv + get.col / p.RT;
+      mbar_arrive_expect_tx(&full[warp][st], S::TILE);
+      tma_load_3d(slots + st * S::TILE, &tmk, &full[warp][st], 0, key0, bh);
+      tma_load_3d(slots + st * S::TILE + KT * D, &tmv, &full[warp][st], 0, key0, bh);
     }
-    const int col = (pos - base) / nt;
-    const int ta = (pos - base) - col * nt;    // first tile of this piece
-    const int n = min(nt - ta, end - pos);     // its tiles
-    const int hk = col / p.RT, rt = col - hk * p.RT;
+    if (--to_get > 0 && ++get.t == get.nt) get.next_column(p, cols);
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES; ++i) load_tile();
+  const float ninf = -INFINITY;
+  int piece = 0;
+
+  for (;;) {
+    const int b = use.b, kv_len = use.kv_len;
+    const int n = min(use.nt - use.t, left);  // tiles of this piece of the column
+    const int hk = use.col / p.RT, rt = use.col - hk * p.RT;
     const int rows = min(ROWS, rows_all - rt * ROWS);
     const int64_t bh = (int64_t)b * p.Hkv + hk;
+    const int key_first = (use.t0 + use.t) * KT;
     const uint8_t* ksb = p.ks + bh * p.nblk;
     const uint8_t* vsb = p.vs + bh * p.nblk;
-    const int my_n = (n - warp + WARPS - 1) / WARPS;                  // tiles of this warp: warp, warp + 4, ...
-    const int key_first = (tl.x + ta + warp) * KT;
-
-    auto load_tile = [&](int i) {  // into the slot that the warp has finished reading
-      const uint32_t st = issued++ % STAGES;
-      if (lane == 0) {
-        const int key0 = key_first + i * (WARPS * KT);
-        mbar_arrive_expect_tx(&full[warp][st], S::TILE);
-        tma_load_3d(slots + st * S::TILE, &tmk, &full[warp][st], 0, key0, (int)bh);
-        tma_load_3d(slots + st * S::TILE + KT * D, &tmv, &full[warp][st], 0, key0, (int)bh);
-      }
-    };
     // scale bytes of a tile's keys: one a 16-key group, or those of this lane's keys g and g + 8
     constexpr int NS = UNI ? U : 2 * U;
     int kbyte[NS], vbyte[NS];
     auto load_scales = [&](int i) {
-      const int key0 = key_first + i * (WARPS * KT);
+      const int key0 = key_first + i * KT;
 #pragma unroll
       for (int x = 0; x < NS; ++x) {
         const int key = UNI ? key0 + x * 16 : key0 + x * 8 + g;
@@ -267,10 +285,7 @@ attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ C
         vbyte[x] = ok ? vsb[key >> p.shift] : kMinScale;
       }
     };
-#pragma unroll
-    for (int i = 0; i < STAGES; ++i)
-      if (i < my_n) load_tile(i);
-    if (my_n > 0) load_scales(0);
+    load_scales(0);
 
     // ---- the queries, scaled to f16: row 8 nt + g of the tile is column g of the nt-th B operand
     uint32_t qb[NT][D / 16][2];
@@ -327,16 +342,16 @@ attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ C
       for (int t = 0; t < MT; ++t) o[nt8][t][0] = o[nt8][t][1] = o[nt8][t][2] = o[nt8][t][3] = 0.f;
     }
 
-    for (int i = 0; i < my_n; ++i) {
+    for (int i = 0; i < n; ++i) {
       int kx[NS], vx[NS];
 #pragma unroll
       for (int x = 0; x < NS; ++x) kx[x] = kbyte[x], vx[x] = vbyte[x];
-      if (i + 1 < my_n) load_scales(i + 1);
+      if (i + 1 < n) load_scales(i + 1);
       const uint32_t st = used % STAGES;
       tile_wait(&full[warp][st], (used / STAGES) & 1, p.status);
       ++used;
       const unsigned char* buf = slots + st * S::TILE;
-      const int key0 = key_first + i * (WARPS * KT);
+      const int key0 = key_first + i * KT;
       // ---- S^T = K Q^T (16 keys x 8 queries an MMA); s[.][u][e]: key 16 u + g + 8 (e >> 1), query 2c + (e & 1)
       float s[NT][U][4];
 #pragma unroll
@@ -493,90 +508,66 @@ attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ C
         }
       }
       __syncwarp();
-      if (i + STAGES < my_n) load_tile(i + STAGES);
+      load_tile();
     }
-    // ---- join the warps through shared memory
-    __syncthreads();
-    float* ow = reinterpret_cast<float*>(ring);
+    // ---- the piece's result: this lane has head dims g * VB .. of the rows 8 nt + 2c, 2c + 1
+    const bool whole = use.t == 0 && n == use.nt;
+    const int64_t slot = (int64_t)me * 2 + (piece > 0);
 #pragma unroll
     for (int nt8 = 0; nt8 < NT; ++nt8)
 #pragma unroll
       for (int q2 = 0; q2 < 2; ++q2) {
         const int r = nt8 * 8 + 2 * c + q2;
+        float L = l[nt8][q2];
 #pragma unroll
-        for (int d = 4; d < 32; d <<= 1) l[nt8][q2] += __shfl_xor_sync(0xffffffffu, l[nt8][q2], d);
-        if (g == 0) wM[warp][r] = limit[nt8][q2] == ninf ? ninf : m[nt8][q2], wL[warp][r] = l[nt8][q2];
-        float4* dst = reinterpret_cast<float4*>(ow + (warp * ROWS + r) * S::OROW + g * VB);
+        for (int d = 4; d < 32; d <<= 1) L += __shfl_xor_sync(0xffffffffu, L, d);
+        if (r >= rows) continue;
+        float x[VB];
 #pragma unroll
-        for (int t = 0; t < MT; t += 2)
-          dst[t / 2] = make_float4(o[nt8][t][q2], o[nt8][t][2 + q2], o[nt8][t + 1][q2], o[nt8][t + 1][2 + q2]);
+        for (int t = 0; t < MT; ++t) x[2 * t] = o[nt8][t][q2], x[2 * t + 1] = o[nt8][t][2 + q2];
+        if (whole) {
+          const float inv = L == 0.f ? 0.f : 1.f / L;
+          uint4* dst = reinterpret_cast<uint4*>(out_row(p, b, hk, rt * ROWS + r, D) + g * VB);
+#pragma unroll
+          for (int k = 0; k < VB / 8; ++k)
+            dst[k] = make_uint4(pack_bf16x2(x[8 * k] * inv, x[8 * k + 1] * inv), pack_bf16x2(x[8 * k + 2] * inv, x[8 * k + 3] * inv),
+                                pack_bf16x2(x[8 * k + 4] * inv, x[8 * k + 5] * inv), pack_bf16x2(x[8 * k + 6] * inv, x[8 * k + 7] * inv));
+        } else {
+          float4* dst = reinterpret_cast<float4*>(p.part + (slot * ROWS + r) * D + g * VB);
+#pragma unroll
+          for (int k = 0; k < VB / 4; ++k) dst[k] = make_float4(x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]);
+          if (g == 0)
+            *reinterpret_cast<float2*>(p.ml + (slot * ROWS + r) * 2) =
+                make_float2(limit[nt8][q2] == ninf ? ninf : m[nt8][q2], L);
+        }
       }
-    __syncthreads();
-    const bool whole = ta == 0 && n == nt;
-    const int64_t slot = (int64_t)blockIdx.x * 2 + (pos != run_first);
-    if (tid < ROWS) {
-      float M = wM[0][tid];
-#pragma unroll
-      for (int w = 1; w < WARPS; ++w) M = fmaxf(M, wM[w][tid]);
-      float L = 0.f;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        const float f = part_weight(wM[w][tid], wL[w][tid], M);
-        L += f == 0.f ? 0.f : f * wL[w][tid];
-        wM[w][tid] = f;
-      }
-      rL[tid] = L;
-      if (!whole && tid < rows) *reinterpret_cast<float2*>(p.ml + (slot * ROWS + tid) * 2) = make_float2(M, L);
-    }
-    __syncthreads();
-    for (int e = tid; e < rows * VB; e += THREADS) {  // 8 head dims of a row
-      const int r = e / VB, d = (e % VB) * 8;
-      float x[8] = {};
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        const float f = wM[w][r];
-        if (f == 0.f) continue;
-        const float4* src = reinterpret_cast<const float4*>(ow + (w * ROWS + r) * S::OROW + d);
-        const float4 u = src[0], v = src[1];
-        x[0] += f * u.x, x[1] += f * u.y, x[2] += f * u.z, x[3] += f * u.w;
-        x[4] += f * v.x, x[5] += f * v.y, x[6] += f * v.z, x[7] += f * v.w;
-      }
-      if (whole) {
-        const float inv = rL[r] == 0.f ? 0.f : 1.f / rL[r];
-        *reinterpret_cast<uint4*>(out_row(p, b, hk, rt * ROWS + r, D) + d) =
-            make_uint4(pack_bf16x2(x[0] * inv, x[1] * inv), pack_bf16x2(x[2] * inv, x[3] * inv),
-                       pack_bf16x2(x[4] * inv, x[5] * inv), pack_bf16x2(x[6] * inv, x[7] * inv));
-      } else {
-        float4* dst = reinterpret_cast<float4*>(p.part + (slot * ROWS + r) * D + d);
-        dst[0] = make_float4(x[0], x[1], x[2], x[3]);
-        dst[1] = make_float4(x[4], x[5], x[6], x[7]);
-      }
-    }
-    fence_proxy_async_smem();  // the merge buffer is the ring, which TMA writes next
-    __syncthreads();
-    pos += n;
+    left -= n;
+    if (left == 0) return;
+    ++piece;
+    use.next_column(p, cols);
   }
 }
 
-// Joins the partials of the columns that several CTAs share, in the order of the CTAs; one CTA a
-// column.  Launched so that everything up to the wait overlaps attend_kernel.
+// Joins the partials of the columns that several warps share, in the order of the list; one CTA
+// for each row of a column.  Launched so that everything up to the wait overlaps attend_kernel.
 template <int D, int NT>
 __global__ void __launch_bounds__(THREADS) join_kernel(AttendParams p) {
-  constexpr int ROWS = 8 * NT, D4 = D / 4, MAXE = ROWS * D4 / THREADS, PER = THREADS / ROWS;
-  extern __shared__ float wt[];  // [partials][ROWS] weights
+  constexpr int ROWS = 8 * NT, D4 = D / 4, GROUPS = THREADS / D4;
+  extern __shared__ __align__(16) float jsm[];  // [JOIN_CHUNK][D] partials, then the weights of all
+  float* wt = jsm + JOIN_CHUNK * D;
   __shared__ int red[WARPS];
-  __shared__ float sL[ROWS];
+  __shared__ float fred[WARPS];
   __shared__ float4 part[THREADS];
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cols = p.Hkv * p.RT;
-  const int b = blockIdx.x / cols, col = blockIdx.x - b * cols;
+  const int b = blockIdx.x / cols, col = blockIdx.x - b * cols, r = blockIdx.y;
   int kl, all = 0, before = 0;
   for (int i = tid; i < p.B; i += THREADS) {
     const int n = tiles_of(p, i, kl).y;
     all += n;
     if (i < b) before += n;
   }
-  const Runs runs(block_sum(all, red) * cols, p.grid);
+  const Runs runs(block_sum(all, red) * cols, p.warps);
   const int nt = tiles_of(p, b, kl).y;
   const int cf = block_sum(before, red) * cols + col * nt;
   grid_dependency_wait();
@@ -584,69 +575,60 @@ __global__ void __launch_bounds__(THREADS) join_kernel(AttendParams p) {
   const int c0 = runs.owner(cf), nc = runs.owner(cf + nt - 1) + 1 - c0;
   if (nc == 1) return;  // written by attend_kernel
   const int hk = col / p.RT, rt = col - hk * p.RT;
-  const int rows = min(ROWS, (p.H / p.Hkv) * p.L - rt * ROWS);
-  // the column is the first piece of every CTA but c0, and of c0 only if c0's run starts with it
+  if (rt * ROWS + r >= (p.H / p.Hkv) * p.L) return;
+  // the column is the first piece of every warp but c0, and of c0 only if its run starts with it
   const bool late = runs.first(c0) != cf;
-  auto slot = [&](int x) { return ((int64_t)c0 + x) * 2 + (x == 0 && late); };
-  {  // rows' maxima, weights and sums: PER threads a row
-    const int r = tid / PER, first = tid % PER;
-    float M = -INFINITY, L = 0.f;
-    if (r < rows)
-#pragma unroll 4
-      for (int x = first; x < nc; x += PER) M = fmaxf(M, p.ml[(slot(x) * ROWS + r) * 2]);
+  auto at = [&](int x) { return (((int64_t)c0 + x) * 2 + (x == 0 && late)) * ROWS + r; };
+  float M = -INFINITY, L = 0.f;
+  for (int x = tid; x < nc; x += THREADS) M = fmaxf(M, p.ml[at(x) * 2]);
 #pragma unroll
-    for (int o = 1; o < PER; o <<= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    if (r < rows)
-      for (int x = first; x < nc; x += PER) {
-        const float2 ml = *reinterpret_cast<const float2*>(p.ml + (slot(x) * ROWS + r) * 2);
-        const float f = part_weight(ml.x, ml.y, M);
-        wt[x * ROWS + r] = f;
-        if (f != 0.f) L += f * ml.y;
-      }
-#pragma unroll
-    for (int o = 1; o < PER; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-    if (first == 0) sL[r] = L;
-  }
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  if (lane == 0) fred[warp] = M;
   __syncthreads();
-  // O as float4 columns; with few rows, groups of threads take every groups-th partial
-  const int n4 = rows * D4, groups = n4 >= THREADS ? 1 : THREADS / n4;
 #pragma unroll
-  for (int k = 0; k < MAXE; ++k) {
-    if (k * THREADS >= n4) break;
-    const int e = groups > 1 ? tid % n4 : k * THREADS + tid, first = groups > 1 ? tid / n4 : 0;
-    const int r = e / D4;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (e < n4 && first < groups) {
-      for (int x0 = first; x0 < nc; x0 += 8 * groups) {  // eight loads at a time
-        float4 v[8];
+  for (int w = 0; w < WARPS; ++w) M = fmaxf(M, fred[w]);
+  __syncthreads();
+  for (int x = tid; x < nc; x += THREADS) {
+    const float2 ml = *reinterpret_cast<const float2*>(p.ml + at(x) * 2);
+    const float f = part_weight(ml.x, ml.y, M);
+    wt[x] = f;
+    if (f != 0.f) L += f * ml.y;
+  }
 #pragma unroll
-        for (int y = 0; y < 8; ++y) {
-          const int x = x0 + y * groups;
-          v[y] = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (x < nc) v[y] = *(reinterpret_cast<const float4*>(p.part + slot(x) * ROWS * D) + e);
-        }
+  for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+  if (lane == 0) fred[warp] = L;
+  __syncthreads();
+  L = 0.f;
 #pragma unroll
-        for (int y = 0; y < 8; ++y) {
-          const float f = wt[min(x0 + y * groups, nc - 1) * ROWS + r];  // v is 0 where f does not belong to it
-          a.x += f * v[y].x, a.y += f * v[y].y, a.z += f * v[y].z, a.w += f * v[y].w;
-        }
-      }
-    }
-    if (groups > 1) {
-      part[tid] = a;
-      __syncthreads();
-      if (tid < n4)
-        for (int x = 1; x < groups; ++x) {
-          const float4 v = part[x * n4 + tid];
-          a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
-        }
-    }
-    if (groups > 1 ? tid < n4 : e < n4) {
-      const float inv = sL[r] == 0.f ? 0.f : 1.f / sL[r];
-      *reinterpret_cast<uint2*>(out_row(p, b, hk, rt * ROWS + r, D) + (e % D4) * 4) =
-          make_uint2(pack_bf16x2(a.x * inv, a.y * inv), pack_bf16x2(a.z * inv, a.w * inv));
+  for (int w = 0; w < WARPS; ++w) L += fred[w];
+  // the partials by asynchronous copies, CHUNK at a time; groups of D / 4 threads sum every GROUPS-th
+  float4* stage = reinterpret_cast<float4*>(jsm);
+  const int e = tid % D4, first = tid / D4;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int x0 = 0; x0 < nc; x0 += JOIN_CHUNK) {
+    const int nb = min(JOIN_CHUNK, nc - x0);
+    for (int x = first; x < nb; x += GROUPS)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(stage + x * D4 + e)),
+                   "l"(p.part + at(x0 + x) * D + e * 4)
+                   : "memory");
+    asm volatile("cp.async.wait_all;" ::: "memory");  // a thread sums what it copied itself
+    for (int x = first; x < nb; x += GROUPS) {
+      const float f = wt[x0 + x];
+      const float4 v = stage[x * D4 + e];
+      a.x = fmaf(f, v.x, a.x), a.y = fmaf(f, v.y, a.y), a.z = fmaf(f, v.z, a.z), a.w = fmaf(f, v.w, a.w);
     }
   }
+  part[tid] = a;
+  __syncthreads();
+  if (tid >= D4) return;
+#pragma unroll
+  for (int x = 1; x < GROUPS; ++x) {
+    const float4 v = part[x * D4 + tid];
+    a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  *reinterpret_cast<uint2*>(out_row(p, b, hk, rt * ROWS + r, D) + e * 4) =
+      make_uint2(pack_bf16x2(a.x * inv, a.y * inv), pack_bf16x2(a.z * inv, a.w * inv));
 }
 
 // Up to this many query rows a KV head (heads of the group x new tokens) take the kernel above,
@@ -717,16 +699,16 @@ torch::Tensor kv8_attend(torch::Tensor q, torch::Tensor keys, torch::Tensor valu
   if (left >= 0) span = std::min<int64_t>(span, left + L + KT);
   const int64_t columns = (int64_t)c.B * c.Hkv * p.RT;
   const int64_t want = (columns * ((span + KT - 1) / KT) + WARPS - 1) / WARPS;
-  const int grid = (int)std::min<int64_t>(want, (int64_t)sms[c.device] * per_sm);
+  const int grid = (int)std::min<int64_t>(want, (int64_t)sms[c.device] * per_sm), warps = grid * WARPS;
   TORCH_CHECK(columns * ((c.cap + KT - 1) / KT) <= INT32_MAX, who, ": too many sequences x heads x keys");
-  // workspace: partials of at most two pieces a CTA
-  const int64_t part = (int64_t)grid * 2 * rows * c.D, ml = (int64_t)grid * 2 * rows * 2;
+  // workspace: partials of at most two pieces a warp
+  const int64_t part = (int64_t)warps * 2 * rows * c.D, ml = (int64_t)warps * 2 * rows * 2;
   auto work = torch::empty({part + ml}, q.options().dtype(at::kFloat));
   p.part = work.data_ptr<float>();
   p.ml = p.part + part;
-  p.grid = grid;
+  p.warps = warps;
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
-  auto start = [&](auto kern, int blocks, int smem, bool overlap, auto... args) {
+  auto start = [&](auto kern, dim3 blocks, int smem, bool overlap, auto... args) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = blocks, cfg.blockDim = THREADS, cfg.dynamicSmemBytes = smem, cfg.stream = st;
     cudaLaunchAttribute attr{};
@@ -756,7 +738,7 @@ torch::Tensor kv8_attend(torch::Tensor q, torch::Tensor keys, torch::Tensor valu
   KV8_CASE(d, n, false, true);  \
   KV8_CASE(d, n, true, false);  \
   KV8_CASE(d, n, true, true);   \
-  if (c.D == d && nt == n) start(join_kernel<d, n>, (int)columns, grid * rows * (int)sizeof(float), true, p)
+  if (c.D == d && nt == n) start(join_kernel<d, n>, dim3((int)columns, std::min(rows, G * L)), (JOIN_CHUNK * d + warps) * (int)sizeof(float), true, p)
   KV8_CASES(64, 1);
   KV8_CASES(64, 2);
   KV8_CASES(128, 1);
