@@ -19,19 +19,21 @@ struct AppendParams {
   int span;                   // blocks that L new tokens can touch
 };
 
-// One warp per (sequence, head, touched block, keys or values): largest magnitude of the new
+// WPU warps per (sequence, head, touched block, keys or values): largest magnitude of the new
 // rows of the block, scale byte, quantised rows.  A block that already holds tokens keeps the
 // larger of its scale and the one the new rows need; if it grows, the old rows are shifted to
 // it (rounding once).  Up to kHeld 16-byte vectors a lane stay in registers between the two
-// passes, longer blocks are read again (from L1 / L2).
+// passes, longer blocks are read again (from L1 / L2).  One warp a unit up to 32 kHeld vectors
+// (16 tokens of 128), else four (13 x 1000 tokens in blocks of 64: 24 us with the read back instead of 33).
 constexpr int kAppendWarps = 4, kHeld = 8;
 
-template <int D, bool INT8>
+template <int D, bool INT8, int WPU>
 __global__ void __launch_bounds__(kAppendWarps * 32) append_kernel(AppendParams p) {
+  constexpr int STEP = 32 * WPU;  // threads of a unit
   // a kernel that attends to the new tokens may start its prologue (and waits for the rest)
   asm volatile("griddepcontrol.launch_dependents;");
-  const int lane = threadIdx.x & 31;
-  int64_t u = (int64_t)blockIdx.x * kAppendWarps + (threadIdx.x >> 5);
+  const int lane = threadIdx.x % STEP;
+  int64_t u = WPU == 1 ? (int64_t)blockIdx.x * kAppendWarps + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
   if (u >= (int64_t)p.B * p.Hkv * p.span * 2) return;
   const int kv = (int)(u & 1);
   u >>= 1;
@@ -60,22 +62,29 @@ __global__ void __launch_bounds__(kAppendWarps * 32) append_kernel(AppendParams 
   };
 #pragma unroll
   for (int i = 0; i < kHeld; ++i)
-    if (lane + 32 * i < nvec) held[i] = load(lane + 32 * i);
+    if (lane + STEP * i < nvec) held[i] = load(lane + STEP * i);
 #pragma unroll
   for (int i = 0; i < kHeld; ++i)
-    if (lane + 32 * i < nvec) look(held[i]);
-  for (int i = lane + 32 * kHeld; i < nvec; i += 32) look(load(i));
-  const uint32_t amax = __reduce_max_sync(0xffffffffu, max(amax2 & 0xffffu, amax2 >> 16));
-  const int need = scale_byte<INT8>(amax);
+    if (lane + STEP * i < nvec) look(held[i]);
+  for (int i = lane + STEP * kHeld; i < nvec; i += STEP) look(load(i));
+  uint32_t amax = __reduce_max_sync(0xffffffffu, max(amax2 & 0xffffu, amax2 >> 16));
   uint8_t* sp = p.scale[kv] + bh * p.nblk + blk;
+  const int old = lo > first ? *sp : 0;
+  if constexpr (WPU > 1) {  // (also: every thread has read the old scale)
+    __shared__ uint32_t wmax[WPU];
+    if ((threadIdx.x & 31) == 0) wmax[threadIdx.x >> 5] = amax;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WPU; ++w) amax = max(amax, wmax[w]);
+  }
+  const int need = scale_byte<INT8>(amax);
   int byte = need;
   if (lo > first) {
-    const int old = *sp;
     byte = max(old, need);
     if (byte > old && byte != kBadScale) {  // the block's maximum rose: old rows to the new scale
       const float f = byte - old > 126 ? 0.f : __int_as_float((127 - (byte - old)) << 23);
       uint2* rows = reinterpret_cast<uint2*>(p.data[kv] + (bh * p.cap + first) * D);
-      for (int i = lane; i < (int)(lo - first) * VR; i += 32) {
+      for (int i = lane; i < (int)(lo - first) * VR; i += STEP) {
         const uint2 w = rows[i];
         uint32_t r[2];
 #pragma unroll
@@ -106,8 +115,8 @@ __global__ void __launch_bounds__(kAppendWarps * 32) append_kernel(AppendParams 
   };
 #pragma unroll
   for (int i = 0; i < kHeld; ++i)
-    if (lane + 32 * i < nvec) store(lane + 32 * i, held[i]);
-  for (int i = lane + 32 * kHeld; i < nvec; i += 32) store(i, load(i));
+    if (lane + STEP * i < nvec) store(lane + STEP * i, held[i]);
+  for (int i = lane + STEP * kHeld; i < nvec; i += STEP) store(i, load(i));
 }
 
 struct ReadParams {
@@ -243,12 +252,17 @@ void append(const Cache& c, torch::Tensor k, torch::Tensor v, const int* seqlens
   p.span = ((L - 2) >> c.shift) + 2;  // 1 for L == 1
   if (L == 1) p.span = 1;
   const int64_t units = (int64_t)c.B * c.Hkv * p.span * 2;
-  const int64_t grid = (units + kAppendWarps - 1) / kAppendWarps;
+  const bool wide = (int64_t)std::min(L, 1 << c.shift) * (c.D / 8) > 32 * kHeld;
+  const int64_t grid = wide ? units : (units + kAppendWarps - 1) / kAppendWarps;
   TORCH_CHECK(grid <= INT32_MAX, who, ": too many blocks to write");
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
   auto launch = [&](auto kern) { kern<<<(int)grid, kAppendWarps * 32, 0, st>>>(p); };
-  pick(c, launch, append_kernel<64, false>, append_kernel<64, true>, append_kernel<128, false>,
-       append_kernel<128, true>);
+  if (wide)
+    pick(c, launch, append_kernel<64, false, kAppendWarps>, append_kernel<64, true, kAppendWarps>,
+         append_kernel<128, false, kAppendWarps>, append_kernel<128, true, kAppendWarps>);
+  else
+    pick(c, launch, append_kernel<64, false, 1>, append_kernel<64, true, 1>, append_kernel<128, false, 1>,
+         append_kernel<128, true, 1>);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 

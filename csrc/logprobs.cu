@@ -15,11 +15,11 @@
 namespace mykb {
 namespace lp {
 
-constexpr int THREADS = 256, WARPS = THREADS / 32;
-constexpr int UN = 4;          // 16-byte vectors a thread loads at a time
+constexpr int THREADS = 256;   // of the gradient kernel
+constexpr int UN = 4;          // 16-byte vectors a thread of it loads at a time
 constexpr int kMaxTop = 32;
 constexpr int kCand = 1024;    // candidates kept for the top alternatives
-constexpr int kSteps = 32;     // loop steps whose maxima a thread remembers
+constexpr int kStepMax = 4096;  // maxima of loop steps that a CTA remembers
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <typename T>
@@ -106,15 +106,19 @@ __device__ __forceinline__ uint32_t warp_merge(uint32_t v, int lane) {  // of a 
   return v;
 }
 
-// One CTA a row, one pass over it.  The row's top k are found from the threads' own maxima: the
+// One CTA a row, one pass over it: 4096 rows of 65536 bf16 logits with 5 alternatives take 127 us
+// (0.65 of the copy bandwidth; two vectors a thread ahead and five CTAs an SM were the best of the
+// depths and occupancies tried, 127 to 208 us), bound by the exponentials and the joins at the
+// ends of rows as much as by the loads.  The row's top k are found from the threads' own maxima: the
 // k-th largest of those is at most the k-th largest logit, so only the few elements that reach
 // it are candidates; threads that have one read those steps of theirs again (from L2), and the
 // candidates are ranked by counting.  Rows with so many equal logits that the candidates do not
 // fit (a mask of -inf over most of the vocabulary) take the larger ones and then the first
 // equal ones in order.
-template <typename T, bool TOP>
-__global__ void __launch_bounds__(THREADS) fwd_kernel(FwdParams<T> p) {
-  constexpr int N = Vec<T>::N;
+template <typename T, bool TOP, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 5 : 1) fwd_kernel(FwdParams<T> p) {
+  constexpr int UN = THREADS == 256 ? 2 : 4;  // vectors a thread loads at a time
+  constexpr int N = Vec<T>::N, WARPS = THREADS / 32, kSteps = kStepMax / THREADS;
   const int64_t row = blockIdx.x;
   const T* x = p.x + row * p.stride;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -134,13 +138,21 @@ __global__ void __launch_bounds__(THREADS) fwd_kernel(FwdParams<T> p) {
   if (tid < head) one(Vec<T>::load(x + tid));
   const int steps = (nvec + THREADS * UN - 1) / (THREADS * UN);
   const uint4 fill = make_uint4(Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf);
-  for (int st = 0; st < steps; ++st) {
-    uint4 w[UN];
+  // the vectors of the next step are loaded while those of this one are summed
+  uint4 next[UN];
+  auto load = [&](int st) {
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
       const int i = (st * UN + u) * THREADS + tid;
-      w[u] = i < nvec ? __ldg(xv + i) : fill;
+      next[u] = i < nvec ? __ldg(xv + i) : fill;
     }
+  };
+  load(0);
+  for (int st = 0; st < steps; ++st) {
+    uint4 w[UN];
+#pragma unroll
+    for (int u = 0; u < UN; ++u) w[u] = next[u];
+    if (st + 1 < steps) load(st + 1);
     float v[UN][N], mx = -INFINITY;
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
@@ -323,7 +335,8 @@ struct BwdParams {
   int V, top, chunk, chunks;
 };
 
-// One CTA per (row, run of `chunk` logits): the dense part, then the given and top tokens of the
+// One CTA per (row, run of `chunk` logits), bound by HBM (4095 rows of 32768 bf16 logits: 94 us for
+// 537 MB, 0.87 of the copy bandwidth): the dense part, then the given and top tokens of the
 // run are written again with their own terms.
 template <typename T>
 __global__ void __launch_bounds__(THREADS) bwd_kernel(BwdParams<T> p) {
@@ -431,8 +444,16 @@ std::vector<torch::Tensor> logprobs_fwd(torch::Tensor logits, torch::Tensor toke
     p.logprob = stats.data_ptr<float>(), p.entropy = p.logprob + rows, p.lse = p.entropy + rows;
     p.top_lp = tl.data_ptr<float>(), p.top_tok = tt.data_ptr<int64_t>();
     p.V = (int)logits.size(1), p.top = (int)top;
-    if (top > 0) fwd_kernel<T, true><<<(int)rows, THREADS, 0, st>>>(p);
-    else fwd_kernel<T, false><<<(int)rows, THREADS, 0, st>>>(p);
+    // few rows: latency counts, a row's loads are spread over four times the threads (8 rows of 65536 bf16
+    // logits: 13 us instead of 15); many rows: several small CTAs an SM overlap one another's ends of rows
+    const bool few = rows <= at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+    if (top > 0) {
+      if (few) fwd_kernel<T, true, 1024><<<(int)rows, 1024, 0, st>>>(p);
+      else fwd_kernel<T, true, 256><<<(int)rows, 256, 0, st>>>(p);
+    } else {
+      if (few) fwd_kernel<T, false, 1024><<<(int)rows, 1024, 0, st>>>(p);
+      else fwd_kernel<T, false, 256><<<(int)rows, 256, 0, st>>>(p);
+    }
   };
   if (logits.scalar_type() == at::kBFloat16) go((const __nv_bfloat16*)logits.data_ptr());
   else go((const float*)logits.data_ptr());
