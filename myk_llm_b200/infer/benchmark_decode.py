@@ -3,6 +3,7 @@
     python -m myk_llm_b200.infer.benchmark_decode                       # 200M + 2 MTP heads
     python -m myk_llm_b200.infer.benchmark_decode --batch 1 8 64 --prompt 2048 --new 256
     python -m myk_llm_b200.infer.benchmark_decode --impl reference      # the reference's own timing
+    python -m myk_llm_b200.infer.benchmark_decode --kv-dtype e4m3 --logprobs 5   # 8-bit caches, alternatives
     torchrun --nproc-per-node 8 --master-addr 127.0.0.1 -m myk_llm_b200.infer.benchmark_decode  # 8 replicas
 
 With several ranks every GPU runs an independent replica (its own model copy, prompts
@@ -45,7 +46,11 @@ def _events():
     return torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
 
 
-def bench_ours(batch: int, prompt: int, new: int, seed: int = 0) -> dict:
+KV_DTYPES = {"bf16": None, "e4m3": torch.float8_e4m3fn, "int8": torch.int8}
+
+
+def bench_ours(batch: int, prompt: int, new: int, seed: int = 0, kv_dtype: str = "bf16", kv_block: int = 16,
+               logprobs: int | None = None) -> dict:
     from ..configuration import apply_overrides, from_dict
     from ..models import MykLLM, ModelConfig
     from .engine import StaticDecoder
@@ -55,7 +60,8 @@ def bench_ours(batch: int, prompt: int, new: int, seed: int = 0) -> dict:
     model = MykLLM(cfg).cuda().eval()  # fp32 masters; every op computes in bf16 (cached bf16 weights)
     gen = torch.Generator(device="cuda").manual_seed(seed)
     prompts = torch.randint(0, cfg.vocab_size, (batch, prompt), device="cuda", generator=gen)
-    dec = StaticDecoder(model, batch_size=batch, max_len=prompt + new + 4)
+    dec = StaticDecoder(model, batch_size=batch, max_len=prompt + new + 4, kv_dtype=KV_DTYPES[kv_dtype],
+                        kv_block=kv_block, logprobs=logprobs)
     dec.generate(prompts, 8, check_every=4)  # warm-up: kernels, graph capture
     torch.cuda.synchronize()
     # prefill alone
@@ -78,7 +84,11 @@ def bench_ours(batch: int, prompt: int, new: int, seed: int = 0) -> dict:
     total_ms = e2.elapsed_time(e3)
     decode_ms = max(st.decode_s * 1e3, 1e-6)
     capture_ms = max(total_ms - st.prefill_s * 1e3 - decode_ms, 0.0)
-    return {"impl": "ours", "batch": batch, "prompt": prompt, "new_tokens": new, "draft_depth": dec.K,
+    extra = {} if kv_dtype == "bf16" else {"kv_dtype": kv_dtype, "kv_block": kv_block}
+    if st.logprobs is not None:
+        extra |= {"logprobs": logprobs, "mean_logprob": st.logprobs.logprobs.mean().item(),
+                  "mean_entropy": st.logprobs.entropy.mean().item()}
+    return {"impl": "ours", "batch": batch, "prompt": prompt, "new_tokens": new, "draft_depth": dec.K, **extra,
             "prefill_ms": prefill_ms, "prefill_tokens_per_s": batch * prompt / (prefill_ms / 1e3),
             "decode_ms": decode_ms, "decode_tokens_per_s": batch * new / (decode_ms / 1e3),
             "graph_capture_ms": capture_ms, "generate_total_ms": total_ms,
@@ -154,6 +164,10 @@ def main(argv: list[str] | None = None) -> None:
     ap.add_argument("--batch", type=int, nargs="+", default=[1, 8, 64])
     ap.add_argument("--prompt", type=int, default=2048)
     ap.add_argument("--new", type=int, default=256)
+    ap.add_argument("--kv-dtype", choices=list(KV_DTYPES), default="bf16", help="type of the attention caches")
+    ap.add_argument("--kv-block", type=int, default=16, help="tokens that share a scale of an 8-bit cache")
+    ap.add_argument("--logprobs", type=int, default=None, metavar="K",
+                    help="log probability, entropy and K alternatives of every emitted token")
     ap.add_argument("--impl", choices=["ours", "reference", "both"], default="ours")
     args = ap.parse_args(argv)
     sys.path.insert(0, ROOT)
@@ -169,7 +183,8 @@ def main(argv: list[str] | None = None) -> None:
     for b in args.batch:
         acc = 0.0
         if args.impl in ("ours", "both"):
-            r = _replicas(bench_ours(b, args.prompt, args.new, seed=rank), world)
+            r = _replicas(bench_ours(b, args.prompt, args.new, seed=rank, kv_dtype=args.kv_dtype,
+                                     kv_block=args.kv_block, logprobs=args.logprobs), world)
             acc = r["acceptance"]
             if rank == 0:
                 print(json.dumps(r), flush=True)

@@ -23,6 +23,13 @@ window (one state read and one write per layer and round).  Looped models get on
 entry per core iteration; n-gram models carry the last ``context`` committed tokens per row
 as the embedding's left context.
 
+With ``kv_dtype`` (e4m3 or int8) the attention caches are held in 8 bits with a scale for
+each ``kv_block`` tokens (``StaticKV8``): half the bytes a round reads, twice the tokens that
+fit.  A rejected draft may then have raised the scale of the block it was in, which coarsens
+that block's other tokens; with ``kv_block=1`` nothing outlives a rejected draft.  With
+``logprobs=k`` every emitted token also gets its log probability, the entropy of its
+distribution and k alternatives (``DecodeStats.logprobs``).
+
 Verification is greedy, so the emitted sequence equals plain greedy decoding of the main
 model.  A round has static shapes and no host synchronisation, so on CUDA it is captured
 once in a CUDA graph and replayed; the host looks at the output only every few rounds.
@@ -35,7 +42,8 @@ from dataclasses import dataclass, field
 
 import torch
 
-from ..models.mixers import DeltaNet, SpecDeltaState, StaticKV
+from .. import ops
+from ..models.mixers import DeltaNet, SpecDeltaState, StaticKV, StaticKV8
 from ..models.transformer import MykLLM
 
 
@@ -48,6 +56,7 @@ class DecodeStats:
     prefill_s: float = 0.0
     decode_s: float = 0.0
     per_depth_accept: list[float] = field(default_factory=list)
+    logprobs: ops.TokenLogprobs | None = None  # of the new tokens, each (batch, new[, k])
 
     @property
     def acceptance(self) -> float:
@@ -63,8 +72,10 @@ class StaticDecoder:
     ``draft_depth > 0`` (default: all of them)."""
 
     def __init__(self, model: MykLLM, batch_size: int, max_len: int, draft_depth: int | None = None,
-                 use_cuda_graph: bool = True) -> None:
+                 use_cuda_graph: bool = True, kv_dtype: torch.dtype | None = None, kv_block: int = 16,
+                 logprobs: int | None = None) -> None:
         cfg = model.config
+        self.logprobs = logprobs
         self.model = model.eval()
         self.cfg = cfg
         self.B, self.cap = batch_size, max_len
@@ -78,6 +89,9 @@ class StaticDecoder:
         cap = max_len + self.K + 2
 
         def kv():
+            if kv_dtype is not None:
+                return StaticKV8(ops.kv8_cache(batch_size, cap, a.num_kv_heads, a.head_dim, dtype=kv_dtype,
+                                               block=kv_block, device=dev), self.seqlens)
             return StaticKV(torch.zeros(batch_size, cap, a.num_kv_heads, a.head_dim, dtype=dt, device=dev),
                             torch.zeros(batch_size, cap, a.num_kv_heads, a.head_dim, dtype=dt, device=dev),
                             self.seqlens)
@@ -125,7 +139,10 @@ class StaticDecoder:
             st.prefill = True
         pos = torch.arange(P, device=self.device).expand(B, -1)
         out = self._main(prompts, pos)
-        y_last = self._head_argmax(out.hidden[:, -1:])[:, 0]
+        logits = self.model.logits(out.hidden[:, -1:])
+        y_last = logits.float().argmax(-1)[:, 0]
+        if self.logprobs is not None:
+            self.first_logprobs = ops.token_logprobs(logits[:, 0], y_last, top=self.logprobs)
         # MTP modules over the prompt: depth k at position i sees token i+k (known inside
         # the prompt, else the greedy token / the previous depth's draft)
         hidden = out.residual
@@ -150,7 +167,8 @@ class StaticDecoder:
         w = torch.cat([self.bonus[:, None], self.drafts], 1)  # (B, K+1)
         pos = self.seqlens.long()[:, None] + self._ar[None, :K + 1]
         out = self._main(w, pos, self.history if self.context else None)
-        y = self._head_argmax(out.hidden)  # (B, K+1)
+        logits = self.model.logits(out.hidden)
+        y = logits.float().argmax(-1)  # (B, K+1)
         if K:
             match = (w[:, 1:] == y[:, :-1]).int()
             a = match.cumprod(1).sum(1)  # accepted drafts per row
@@ -165,6 +183,9 @@ class StaticDecoder:
         valid = self._ar[None, :K + 1] <= a[:, None]
         cols = torch.where(valid, cols, torch.full_like(cols, self.out_tokens.size(1) - 1))
         self.out_tokens.scatter_(1, cols.clamp(max=self.out_tokens.size(1) - 1), torch.where(valid, emit, self._pad))
+        if self.logprobs is not None:  # the i-th token emitted this round is y[:, i]
+            for buf, x in zip(self.out_logprobs, ops.token_logprobs(logits, y, top=self.logprobs)):
+                buf.scatter_(1, cols.clamp(max=buf.size(1) - 1).view(*cols.shape, *[1] * (x.dim() - 2)).expand(x.shape), x)
         self.out_len += a + 1
         self.acc_sum += a
         if K:
@@ -217,6 +238,10 @@ class StaticDecoder:
         self._pad = torch.zeros((), dtype=torch.long, device=self.device)
         self.out_tokens = torch.zeros(B, max_new_tokens + self.K + 2, dtype=torch.long, device=self.device)
         self.out_tokens[:, 0] = self.bonus
+        if self.logprobs is not None:
+            self.out_logprobs = [x.new_zeros(B, self.out_tokens.size(1), *x.shape[1:]) for x in self.first_logprobs]
+            for buf, x in zip(self.out_logprobs, self.first_logprobs):
+                buf[:, 0] = x
         self.out_len = torch.ones(B, dtype=torch.long, device=self.device)
         self.acc_sum = torch.zeros(B, dtype=torch.long, device=self.device)
         self.acc_depth = torch.zeros(max(1, self.K), dtype=torch.long, device=self.device)
@@ -238,6 +263,8 @@ class StaticDecoder:
         st.accepted_drafts = int(self.acc_sum.sum())
         st.drafted = rounds * B * self.K
         st.per_depth_accept = (self.acc_depth.float() / max(1, rounds * B)).tolist() if self.K else []
+        if self.logprobs is not None:
+            st.logprobs = ops.TokenLogprobs(*(x[:, :max_new_tokens].clone() for x in self.out_logprobs))
         toks = torch.cat([prompts, self.out_tokens[:, :max_new_tokens]], 1)
         return toks, st
 
@@ -246,6 +273,8 @@ class StaticDecoder:
         beyond ``seqlens`` and are harmless to repeat)."""
         out = [self.seqlens, self.pending, self.history, self.bonus, self.drafts, self.out_tokens, self.out_len,
                self.acc_sum, self.acc_depth]
+        if self.logprobs is not None:
+            out += self.out_logprobs
         for st in self.delta_states:
             out += [st.recurrent, *st.inputs] + ([st.conv, st.window_x] if st.conv is not None else [])
         return out

@@ -54,6 +54,14 @@ class StaticKV:
     seqlens: torch.Tensor
 
 
+@dataclass
+class StaticKV8:
+    """``StaticKV`` with the keys and values held in 8 bits (``ops.KVCache8``)."""
+
+    cache: ops.KVCache8
+    seqlens: torch.Tensor
+
+
 class Attention(nn.Module):
     """Grouped-query causal softmax attention, global or sliding-window."""
 
@@ -99,6 +107,10 @@ class Attention(nn.Module):
         if isinstance(state, StaticKV):
             out = ops.flash_attn_with_kvcache(q, state.keys, state.values, k, v, cache_seqlens=state.seqlens,
                                               causal=True, window_size=window)
+            new_state = state
+        elif isinstance(state, StaticKV8):
+            out = ops.flash_attn_with_kvcache8(q, state.cache, k, v, cache_seqlens=state.seqlens, causal=True,
+                                               window_size=window)
             new_state = state
         elif varlen is not None:
             out = ops.flash_attn_varlen_func(
@@ -149,6 +161,9 @@ class SharedKV(nn.Module):
             state.keys[rows, cols] = k
             state.values[rows, cols] = v
             return state
+        if isinstance(state, StaticKV8):
+            ops.kv8_append(state.cache, k, v, cache_seqlens=state.seqlens)
+            return state
         if state is not None:
             k = torch.cat([state.keys, k], dim=1)
             v = torch.cat([state.values, v], dim=1)
@@ -191,6 +206,8 @@ class CrossAttention(nn.Module):
         if isinstance(kv, StaticKV):
             return ops.flash_attn_with_kvcache(q, kv.keys, kv.values, cache_seqlens=kv.seqlens + q.shape[1],
                                                causal=True)
+        if isinstance(kv, StaticKV8):
+            return ops.flash_attn_with_kvcache8(q, kv.cache, cache_seqlens=kv.seqlens + q.shape[1], causal=True)
         if varlen is None:
             return ops.flash_attn_func(q, kv.keys, kv.values, causal=True)
         return ops.flash_attn_varlen_func(
