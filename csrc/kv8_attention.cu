@@ -631,10 +631,19 @@ __global__ void __launch_bounds__(THREADS) join_kernel(AttendParams p) {
       make_uint2(pack_bf16x2(a.x * inv, a.y * inv), pack_bf16x2(a.z * inv, a.w * inv));
 }
 
-// Up to this many query rows a KV head (heads of the group x new tokens) take the kernel above,
-// whose 16-row tiles each walk the cache; more rows read the cache back to bf16 once and take
-// the prefill kernel.
-constexpr int kMaxRows = 64;
+// Whether to read the cache back to bf16 and run the prefill kernel instead.  attend_kernel takes
+// about 0.05 ns a key and column (0.037 at head_dim 64: its tiles come from L2 after the first row
+// tile); the prefill kernel 20 ns a key for each wave of its (128 queries, head) items over the
+// SMs, which is all it is split over, plus the read back at HBM speed.  Measured, us: 1 x 512
+// queries, 16/4 heads of 128, 2048 keys: 72 here, 48 there; 4 x 509, 4096 keys: 384, 88; 8 x 32,
+// 8192 keys: 100, 313; 13 x 155 queries of one head, 30000 keys: 162, 627; 64 x 64, 16/4 heads of
+// 64, 2048 keys: 298, 507.  Up to 64 rows a KV head always stay here.
+static bool prefer_prefill(const Cache& c, int H, int L, int64_t columns, int64_t span, int sms) {
+  const double here = (c.D == 64 ? 0.037 : 0.05) * columns * span;
+  const int64_t items = (int64_t)c.B * H * ((L + 127) / 128);
+  const double there = 20.0 * ((items + sms - 1) / sms) * span + 0.0016 * c.D * c.B * c.Hkv * c.cap;
+  return (int64_t)(H / c.Hkv) * L > 64 && (there < here || columns * ((c.cap + KT - 1) / KT) > INT32_MAX);
+}
 
 }  // namespace kv8
 
@@ -671,7 +680,13 @@ torch::Tensor kv8_attend(torch::Tensor q, torch::Tensor keys, torch::Tensor valu
   if (c.cap == 0) return o.zero_();
   left = left < 0 ? -1 : std::min<int64_t>(left, 1 << 29);
   right = right < 0 ? -1 : std::min<int64_t>(right, 1 << 29);
-  if ((int64_t)G * L > kMaxRows) {
+  static int sms[64] = {0};
+  if (!sms[c.device]) C10_CUDA_CHECK(cudaDeviceGetAttribute(&sms[c.device], cudaDevAttrMultiProcessorCount, c.device));
+  const int nt = G * L <= 8 ? 1 : 2, rows = 8 * nt, RT = (G * L + rows - 1) / rows;
+  int64_t span = c.cap;  // most keys a sequence can show
+  if (left >= 0) span = std::min<int64_t>(span, left + L + KT);
+  const int64_t columns = (int64_t)c.B * c.Hkv * RT;
+  if (prefer_prefill(c, H, L, columns, span, sms[c.device])) {
     auto opt = q.options();
     auto kb = torch::empty({c.B, c.cap, c.Hkv, c.D}, opt), vb = torch::empty({c.B, c.cap, c.Hkv, c.D}, opt);
     read(c, lens, extra, nullptr, 0, c.cap, 256, kb, vb, who);  // 256: more than a key tile of the prefill kernel
@@ -686,18 +701,12 @@ torch::Tensor kv8_attend(torch::Tensor q, torch::Tensor keys, torch::Tensor valu
   p.seqlens = lens;
   p.o = (bf16*)o.data_ptr();
   p.q_sb = q.stride(0), p.q_st = q.stride(1), p.q_sh = q.stride(2);
-  const int nt = G * L <= 8 ? 1 : 2, rows = 8 * nt;
-  p.B = c.B, p.L = L, p.H = H, p.Hkv = c.Hkv, p.RT = (G * L + rows - 1) / rows;
+  p.B = c.B, p.L = L, p.H = H, p.Hkv = c.Hkv, p.RT = RT;
   p.cap = c.cap, p.nblk = c.nblk, p.shift = c.shift, p.extra = extra;
   p.left = (int)left, p.right = (int)right;
   p.scale_log2 = (float)(std::abs(scale) * 1.4426950408889634), p.sign = scale < 0 ? -1.f : 1.f;
-  static int sms[64] = {0};
-  if (!sms[c.device]) C10_CUDA_CHECK(cudaDeviceGetAttribute(&sms[c.device], cudaDevAttrMultiProcessorCount, c.device));
   const int per_sm = c.D == 64 ? (nt == 1 ? Shape<64, 1>::PER_SM : Shape<64, 2>::PER_SM)
                                : (nt == 1 ? Shape<128, 1>::PER_SM : Shape<128, 2>::PER_SM);
-  int64_t span = c.cap;  // most keys a sequence can show
-  if (left >= 0) span = std::min<int64_t>(span, left + L + KT);
-  const int64_t columns = (int64_t)c.B * c.Hkv * p.RT;
   const int64_t want = (columns * ((span + KT - 1) / KT) + WARPS - 1) / WARPS;
   const int grid = (int)std::min<int64_t>(want, (int64_t)sms[c.device] * per_sm), warps = grid * WARPS;
   TORCH_CHECK(columns * ((c.cap + KT - 1) / KT) <= INT32_MAX, who, ": too many sequences x heads x keys");

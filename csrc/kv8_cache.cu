@@ -127,7 +127,7 @@ struct ReadParams {
   const int* start;      // (B) or null
   int start0, extra;
   int B, Hkv, cap, nblk, shift, length;
-  int pad;               // >= 0: nothing is written from round-up(length held) + pad on
+  int pad;               // >= 0: for the prefill kernel (see read() in kv8_host.h)
 };
 
 // 16 values a thread and step (16 bytes in, 32 out).  A CTA walks kReadTokens tokens of one
@@ -149,6 +149,7 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(ReadParams p) {
   const uint8_t* src = (kv ? p.data[1] : p.data[0]) + bh * p.cap * D;
   const uint8_t* sc = (kv ? p.scale[1] : p.scale[0]) + bh * p.nblk;
   bf16* out = (kv ? p.out[1] : p.out[0]) + ((int64_t)b * p.length * p.Hkv + h) * D;
+  const uint8_t* sc2 = (kv ? p.scale[0] : p.scale[1]) + bh * p.nblk;  // of the other tensor
   uint4 w[kReadSteps];
   int sb[kReadSteps];
 #pragma unroll
@@ -160,6 +161,10 @@ __global__ void __launch_bounds__(kReadThreads) read_kernel(ReadParams p) {
     if (t < p.length && pos >= 0 && pos < held) {
       w[s] = __ldcs(reinterpret_cast<const uint4*>(src + pos * D + (e % CR) * 16));
       sb[s] = sc[pos >> p.shift];
+      if (p.pad >= 0) {
+        if (kv && sb[s] == kBadScale) sb[s] = kMinScale, w[s] = make_uint4(0, 0, 0, 0);
+        if (!kv && sc2[pos >> p.shift] == kBadScale) sb[s] = kBadScale;
+      }
     }
   }
 #pragma unroll

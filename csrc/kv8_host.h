@@ -28,7 +28,9 @@ void check_lens(const torch::Tensor& t, const Cache& c, const torch::Tensor& key
 void append(const Cache& c, torch::Tensor k, torch::Tensor v, const int* seqlens, const char* who);
 
 // bf16 copies (B, length, Hkv, D) of tokens start[b] (or start0) onward; tokens from seqlens[b] + extra on are 0.
-// pad >= 0: the part of the copy that lies more than `pad` tokens past them is left unwritten.
+// pad >= 0: for an attention kernel that multiplies masked values by 0: the part of the copy that lies more
+// than `pad` tokens past them is left unwritten, and a block marked as bad in either tensor gets NaN keys (whose
+// scores the mask replaces) and values of 0 instead of NaN.
 void read(const Cache& c, const int* seqlens, int extra, const int* start, int start0, int length, int pad,
           torch::Tensor& k, torch::Tensor& v, const char* who);
 

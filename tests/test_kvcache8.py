@@ -235,7 +235,7 @@ ATTEND = [
     ((1500, 3, 0, 700), 3, True, 16, 4, 64, 16, True, (-1, -1)),
     ((513, 100, 2), 1, False, 8, 2, 128, 64, True, (511, 0)),
     ((90, 1000), 5, True, 6, 2, 64, 1, True, (40, 0)),
-    ((77, 4), 9, True, 8, 1, 128, 8, True, (-1, -1)),          # 72 rows: read back, prefill kernel
+    ((77, 4), 9, True, 8, 1, 128, 8, True, (-1, -1)),          # 72 rows: five row tiles
     ((77, 4), 6, True, 8, 1, 128, 8, True, (-1, -1)),          # 48 rows: three row tiles
     ((3, 10), 8, False, 2, 2, 64, 32, True, (-1, -1)),         # more queries than keys: empty rows
     ((200, 50), 4, False, 4, 4, 128, 16, False, (-1, -1)),     # bidirectional
@@ -293,6 +293,45 @@ def test_attend_gpu(case, dtype):
 
     _attend_case("cuda", case, dtype)
     assert ops.ext().take_status() == 0
+
+
+PREFILL = [  # wide enough that the cache is read back for the prefill kernel
+    ((100, 0, 3000), 600, True, 16, 4, 128, 16, True, (-1, -1)),
+    ((700, 31), 601, False, 16, 4, 64, 8, True, (-1, -1)),
+    ((100,), 1030, True, 8, 2, 128, 64, True, (200, 0)),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+@pytest.mark.parametrize("case", PREFILL)
+def test_attend_prefill_gpu(case, dtype):
+    from myk_llm_b200 import ops
+
+    _attend_case("cuda", case, dtype)
+    assert ops.ext().take_status() == 0
+
+
+@pytest.mark.gpu
+def test_prefill_nan_only_where_seen():
+    """As test_attend_nan_only_where_seen, through the prefill kernel: earlier queries of the same
+    tile and queries whose window has passed the block stay finite, for a bad key or value."""
+    from myk_llm_b200 import ops
+
+    b, n, new, hk, d = 2, 900, 700, 2, 64
+    q = _data((b, new, 8, d), 3, "cuda")
+    zero = torch.zeros(b, dtype=torch.int32, device="cuda")
+    at = torch.arange(n - new, n, device="cuda")
+    for bad in (0, 1):
+        kv = [_data((b, n, hk, d), 1, "cuda"), _data((b, n, hk, d), 2, "cuda")]
+        kv[bad][0, 300, 1, 5] = math.nan  # tokens 288 .. 303 of sequence 0, head 1
+        cache = ops.kv8_cache(b, 960, hk, d, block=16, device="cuda")
+        ops.kv8_append(cache, *kv, cache_seqlens=zero)
+        for left in (-1, 99):
+            out = ops.flash_attn_with_kvcache8(q, cache, cache_seqlens=zero + n, causal=True, window_size=(left, 0))
+            sees = (at >= 288) & ((at - left <= 303) if left >= 0 else (at >= 0))
+            assert out[0, sees, 4:].isnan().all() and not out[0, ~sees, 4:].isnan().any()
+            assert not out[0, :, :4].isnan().any() and not out[1].isnan().any()
 
 
 @pytest.mark.gpu
