@@ -12,18 +12,24 @@
 // rescaled only when a row's maximum grows by more than 2^7.  Sums, maxima and O are fp32.
 //
 // A decode step reads every visible byte of the cache once and does little with it, so it is
-// bound by HBM.  One work list holds the 16-key-multiple tiles of all (sequence, KV head,
-// row tile) columns; every warp takes an equal run of it, computed on the device from the
-// lengths (ragged batches stay balanced, a captured CUDA graph stays valid).  Every warp has a run
-// of its own, which it reads through a ring of its own that TMA fills (32 keys and 32 values a
-// tile, two bulk copies), running ahead over the ends of columns; warps never wait for one
-// another.  Keys are the M
-// side of Q K^T and head dims that of P V, so that one 8-column tile holds up to 8 query rows;
-// the contraction index of the first and the row index of the second are permuted to make a
-// lane's bytes contiguous in shared memory.
+// bound by HBM.  One work list holds the 32-key tiles of all (sequence, KV head, row tile)
+// columns; every warp takes an equal run of it, computed on the device from the lengths (ragged
+// batches stay balanced, a captured CUDA graph stays valid), and reads it through a ring of its
+// own that TMA fills (two bulk copies a tile), running ahead over the ends of columns; warps
+// never wait for one another.  Keys are the M side of Q K^T and head dims that of P V, so that
+// one 8-column tile holds up to 8 query rows; the contraction index of the first and the row
+// index of the second are permuted to make a lane's bytes contiguous in shared memory.
 // A column that one warp covers is written at once; else the warps leave fp32 partials and a
 // second kernel, whose start overlaps the first, joins them in order: no atomics, and results
 // that do not depend on timing.
+//
+// Measured (B200, CUDA graph, both kernels): 64 sequences of 8192 tokens, 16/4 heads of 128, e4m3:
+// 95.5 us, 0.86 of the copy bandwidth (per-lane asynchronous copies instead of TMA: 117 us, of
+// which the loads alone took 116).  Two sequences of 131071 tokens: 59.5 us, 0.69 (the join of 222
+// partials a column is 10 us of it).  Small calls are bound by latency: one sequence of 2048
+// tokens 9.2 us, 48 sequences that see 512 tokens 11.6 us.  Three queries a sequence (two MMA
+// columns a row tile, 12 warps an SM): bound by the chain QK -> exp -> PV of each warp's few
+// tiles, 64 ragged sequences of up to 2048 tokens 28 us for 31 MB.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
