@@ -697,6 +697,12 @@ torch::Tensor kv8_attend(torch::Tensor q, torch::Tensor keys, torch::Tensor valu
     auto kb = torch::empty({c.B, c.cap, c.Hkv, c.D}, opt), vb = torch::empty({c.B, c.cap, c.Hkv, c.D}, opt);
     read(c, lens, extra, nullptr, 0, c.cap, 256, kb, vb, who);  // 256: more than a key tile of the prefill kernel
     auto used = (seqlens + extra).clamp_(0, c.cap);
+    // the prefill kernel takes the maximum of the scores before it scales them, so its scale must be
+    // positive: a sign goes into the queries (exactly), and so does a 0 (an infinity or NaN becomes NaN)
+    if (scale <= 0) {
+      q = scale < 0 ? q.neg() : q.mul(0);
+      scale = scale < 0 ? -scale : 1.0;
+    }
     return fa_fwd(rows16(q) ? q : q.clone(at::MemoryFormat::Contiguous), kb, vb, c10::nullopt, c10::nullopt, used, L, c.cap, scale,
                   left, right)[0];
   }

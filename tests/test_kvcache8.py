@@ -482,6 +482,41 @@ def test_offsets_past_32_bits():
     assert bool(((out[-1:].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * mag).all())
 
 
+SCALES = [  # (lengths before, new, appended, heads, kv_heads, d, block, window): wide enough for the prefill kernel
+    ((100, 0, 700), 600, True, 8, 2, 64, 16, (-1, -1)),
+    ((300, 41), 515, False, 8, 2, 128, 8, (99, 0)),
+    ((900,), 1100, True, 12, 4, 64, 64, (1200, 0)),  # an odd number of query heads a KV head
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [-0.125, 0.0])
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+@pytest.mark.parametrize("case", SCALES)
+def test_attend_prefill_scale_not_positive(case, dtype, scale):
+    """Negative and zero softmax scales in calls as wide as a prompt, under causal and window masks."""
+    from myk_llm_b200 import ops
+
+    lens, new, step, heads, hk, d, block, window = case
+    b, cap = len(lens), max(lens) + new + 5
+    cache, plain = _cache(b, cap, hk, d, dtype, block, "cuda")
+    held = [_data((b, cap, hk, d), s, "cuda", spread=False) for s in (1, 2)]
+    zero = torch.zeros(b, dtype=torch.int32, device="cuda")
+    ops.kv8_append(cache, *held, cache_seqlens=zero)
+    for p, x in zip(plain, held):
+        p.append(x, [0] * b)
+    q = _data((b, new, heads, d), 3, "cuda") * 0.5
+    kv = [_data((b, new, hk, d), s, "cuda", spread=False) for s in (4, 5)] if step else []
+    out = ops.flash_attn_with_kvcache8(q, cache, *kv, cache_seqlens=zero + torch.tensor(lens, device="cuda"), causal=True,
+                                       window_size=window, softmax_scale=scale)
+    for p, x in zip(plain, kv):
+        p.append(x, lens)
+    total = [n + new if step else n for n in lens]
+    want, mag = _attend(q, plain[0].values(), plain[1].values(), total, window[0], 0, scale)
+    assert bool(((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -7 * mag).all())
+    assert ops.ext().take_status() == 0
+
+
 # ------------------------------------------------------------------------- refusals
 def test_cache_refusals():
     from myk_llm_b200 import ops
