@@ -703,8 +703,11 @@ torch::Tensor kv8_attend(torch::Tensor q, torch::Tensor keys, torch::Tensor valu
       q = scale < 0 ? q.neg() : q.mul(0);
       scale = scale < 0 ? -scale : 1.0;
     }
-    return fa_fwd(rows16(q) ? q : q.clone(at::MemoryFormat::Contiguous), kb, vb, c10::nullopt, c10::nullopt, used, L, c.cap, scale,
-                  left, right)[0];
+    // it reads queries as rows of packed heads, equally far apart over the whole batch
+    const bool packed = rows16(q) && (H == 1 || q.stride(2) == c.D) && q.stride(1) >= (int64_t)H * c.D &&
+                        (c.B == 1 || q.stride(0) == L * q.stride(1));
+    if (!packed) q = q.clone(at::MemoryFormat::Contiguous);
+    return fa_fwd(q, kb, vb, c10::nullopt, c10::nullopt, used, L, c.cap, scale, left, right)[0];
   }
   if (!rows16(q)) q = q.clone(at::MemoryFormat::Contiguous);
   AttendParams p{};

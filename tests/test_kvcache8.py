@@ -517,6 +517,43 @@ def test_attend_prefill_scale_not_positive(case, dtype, scale):
     assert ops.ext().take_status() == 0
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [4, 600])
+def test_attend_query_layouts(new):
+    """Queries laid out head by head, as a chunk of a longer batch of tokens, as heads of a fused projection and
+    shared by the batch, for few and for many rows: the same bits as contiguous ones, and the new tokens in the cache."""
+    from myk_llm_b200 import ops
+
+    b, n, hk, heads, d = 2, 300, 2, 8, 64
+    k, v = (_data((b, n + new, hk, d), s, "cuda") for s in (1, 2))
+    zero = torch.zeros(b, dtype=torch.int32, device="cuda")
+    q = _data((b, new, heads, d), 3, "cuda")
+
+    def call(x, window):
+        cache = ops.kv8_cache(b, n + new, hk, d, device="cuda")
+        ops.kv8_append(cache, k[:, :n], v[:, :n], cache_seqlens=zero)
+        out = ops.flash_attn_with_kvcache8(x, cache, k[:, n:], v[:, n:], cache_seqlens=zero + n, causal=True,
+                                           window_size=window)
+        return out, *ops.kv8_read(cache, cache_seqlens=zero + n + new)
+
+    wide = torch.zeros(b, new + 70, heads, d, dtype=torch.bfloat16, device="cuda")
+    wide[:, 33:33 + new] = q
+    fused = torch.zeros(b, new, heads + 2 * hk, d, dtype=torch.bfloat16, device="cuda")
+    fused[:, :, :heads] = q
+    gaps = torch.zeros(b, new, heads, 2 * d, dtype=torch.bfloat16, device="cuda")
+    gaps[..., :d] = q
+    layouts = [q.transpose(1, 2).contiguous().transpose(1, 2), wide[:, 33:33 + new], fused[:, :, :heads], gaps[..., :d],
+               q.transpose(0, 1).contiguous().transpose(0, 1), q.transpose(2, 3).contiguous().transpose(2, 3)]
+    for window in ((-1, -1), (99, 0)):
+        want = call(q, window)
+        for x in layouts:
+            assert not x.is_contiguous() and torch.equal(x, q)
+            assert all(torch.equal(a, c) for a, c in zip(call(x, window), want))
+        want = call(q[:1].repeat(b, 1, 1, 1), window)
+        assert all(torch.equal(a, c) for a, c in zip(call(q[:1].expand(b, -1, -1, -1), window), want))
+    assert ops.ext().take_status() == 0
+
+
 # ------------------------------------------------------------------------- refusals
 def test_cache_refusals():
     from myk_llm_b200 import ops
