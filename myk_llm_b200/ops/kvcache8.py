@@ -98,15 +98,11 @@ def flash_attn_with_kvcache8(q: torch.Tensor, cache: KVCache8, k: torch.Tensor |
     scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(q.shape[-1])
     left, right = _window(causal, window_size)
     if not q.is_cuda:
-        used = cache_seqlens
+        used = cache_seqlens.clamp(min=0)
         if k is not None and v is not None:
             kv8_append(cache, k, v, cache_seqlens=cache_seqlens)
-            used = cache_seqlens + k.shape[1]
-        used = used.clamp(max=cache.keys.shape[2])
-        keys = ref.kv8_values(cache.keys, cache.key_scales, cache.block).transpose(1, 2)
-        values = ref.kv8_values(cache.values, cache.value_scales, cache.block).transpose(1, 2)
-        out, _ = ref.attention_ref(q, keys, values, causal=causal, window=(left, right), softmax_scale=scale,
-                                   seqused_k=used)
-        return out
+            used = used + k.shape[1]
+        return ref.kv8_attention_ref(q, cache.keys, cache.key_scales, cache.values, cache.value_scales, cache.block,
+                                     used.clamp(max=cache.keys.shape[2]), (left, right), scale)
     return ext().kv8_attend(q, cache.keys, cache.values, cache.key_scales, cache.value_scales, cache.block, k, v,
                             _int32(cache_seqlens), float(scale), left, right)

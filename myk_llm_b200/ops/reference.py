@@ -156,6 +156,32 @@ def kv8_read_ref(data, scales, block, seqlens, start, length):
     return out
 
 
+def kv8_attention_ref(q, keys, key_scales, values, value_scales, block, seqused, window, softmax_scale):
+    """q (B, L, H, D) over a cache; window (left, right) as the kernels take it (right 0: causal).  A row
+    that sees a bad block of keys or values, or has a NaN itself, is NaN; one that sees no key is 0."""
+    bad = ((key_scales == KV8_BAD) | (value_scales == KV8_BAD)).repeat_interleave(block, 2)  # (B, Hkv, cap or more)
+    k, v = kv8_values(keys, key_scales, block), kv8_values(values, value_scales, block)
+    group = q.shape[2] // keys.shape[1]
+    out = torch.zeros(q.shape, dtype=torch.float32, device=q.device)
+    for b, n in enumerate(seqused.tolist()):
+        if n <= 0:
+            continue
+        at = torch.arange(n - q.shape[1], n, device=q.device)[:, None]
+        j = torch.arange(n, device=q.device)[None]
+        seen = torch.ones(q.shape[1], n, dtype=torch.bool, device=q.device)
+        if window[0] >= 0:
+            seen &= j >= at - window[0]
+        if window[1] >= 0:
+            seen &= j <= at + window[1]
+        hit = bad[b, :, :n]  # their NaN goes into the scores, where the mask keeps it from rows that do not see it
+        kb, vb = (x[b, :, :n].masked_fill(hit[..., None], 0.0).repeat_interleave(group, 0) for x in (k, v))
+        s = torch.einsum("qhd,hkd->hqk", q[b].float(), kb) * softmax_scale
+        s = s.masked_fill(hit.repeat_interleave(group, 0)[:, None], math.nan).masked_fill(~seen, -math.inf)
+        live = seen.any(-1)
+        out[b, live] = torch.einsum("hqk,hkd->qhd", torch.softmax(s[:, live], -1), vb)
+    return out.to(q.dtype)
+
+
 # ---------------------------------------------------------------------------------------
 # elementwise / normalisation
 # ---------------------------------------------------------------------------------------

@@ -554,6 +554,68 @@ def test_attend_query_layouts(new):
     assert ops.ext().take_status() == 0
 
 
+def _bad_blocks(device, new):
+    """NaN exactly for the queries that see a bad block, for a bad key and a bad value, with and without a window,
+    and the other rows as if the block were sound."""
+    from myk_llm_b200 import ops
+
+    b, n, hk, d = 2, 64, 2, 64
+    q = _data((b, new, 4, d), 3, device) * 0.5
+    zero = torch.zeros(b, dtype=torch.int32, device=device)
+    at = torch.arange(n - new, n, device=device)
+    for bad, token in ((0, 40), (1, 40), (0, 63), (1, 63), (0, 3), (1, 3)):
+        kv = [_data((b, n, hk, d), s, device, spread=False) for s in (1, 2)]
+        caches = []
+        for spoil in (False, True):
+            if spoil:
+                kv[bad][1, token, 0, 7] = math.nan if token != 3 else -math.inf
+            caches.append(ops.kv8_cache(b, n + 9, hk, d, block=16, device=device))
+            ops.kv8_append(caches[-1], *kv, cache_seqlens=zero)
+        lo = token // 16 * 16
+        for left in (-1, 20):
+            want, got = (ops.flash_attn_with_kvcache8(q, c, cache_seqlens=zero + n, causal=True, window_size=(left, 0))
+                         for c in caches)
+            sees = (at >= lo) & ((at - left <= lo + 15) if left >= 0 else (at >= 0))
+            assert got[1, sees, :2].isnan().all() and not got[1, ~sees, :2].isnan().any()
+            for a, c in ((got[0], want[0]), (got[1, :, 2:], want[1, :, 2:]), (got[1, ~sees, :2], want[1, ~sees, :2])):
+                assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("new", [1, 20, 64])
+def test_bad_blocks_cpu(new):
+    _bad_blocks("cpu", new)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 20, 64])
+def test_bad_blocks_gpu(new):
+    _bad_blocks("cuda", new)
+
+
+def _bad_queries(device):
+    """A NaN in a query makes that row of that head NaN and no other; a row that sees nothing stays 0."""
+    from myk_llm_b200 import ops
+
+    b, n, new, hk, d = 2, 30, 40, 1, 64
+    cache = ops.kv8_cache(b, n, hk, d, device=device)
+    zero = torch.zeros(b, dtype=torch.int32, device=device)
+    ops.kv8_append(cache, _data((b, n, hk, d), 1, device), _data((b, n, hk, d), 2, device), cache_seqlens=zero)
+    q = _data((b, new, 2, d), 3, device)
+    q[1, 35, 0, 3] = math.nan
+    q[0, 5, 1, 3] = math.nan  # ten tokens before the first: sees nothing
+    out = ops.flash_attn_with_kvcache8(q, cache, cache_seqlens=zero + n, causal=True)
+    assert out[1, 35, 0].isnan().all() and out.isnan().sum() == d and not out[:, :10].any()
+
+
+def test_bad_queries_cpu():
+    _bad_queries("cpu")
+
+
+@pytest.mark.gpu
+def test_bad_queries_gpu():
+    _bad_queries("cuda")
+
+
 # ------------------------------------------------------------------------- refusals
 def test_cache_refusals():
     from myk_llm_b200 import ops
