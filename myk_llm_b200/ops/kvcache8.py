@@ -98,8 +98,10 @@ def flash_attn_with_kvcache8(q: torch.Tensor, cache: KVCache8, k: torch.Tensor |
     scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(q.shape[-1])
     left, right = _window(causal, window_size)
     if not q.is_cuda:
+        if (k is None) != (v is None):
+            raise ValueError("new keys and values come together")
         used = cache_seqlens.clamp(min=0)
-        if k is not None and v is not None:
+        if k is not None:
             kv8_append(cache, k, v, cache_seqlens=cache_seqlens)
             used = used + k.shape[1]
         return ref.kv8_attention_ref(q, cache.keys, cache.key_scales, cache.values, cache.value_scales, cache.block,

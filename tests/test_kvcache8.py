@@ -634,6 +634,19 @@ def test_cache_refusals():
         ops.kv8_read(cache, cache_seqlens=torch.ones(1), length=-1)
 
 
+def test_attend_new_keys_and_values_together_cpu():
+    """As on the GPU, new keys without values (or the reverse) are refused and nothing is written."""
+    from myk_llm_b200 import ops
+
+    cache = ops.kv8_cache(1, 8, 1, 64)
+    x = torch.ones(1, 1, 1, 64)
+    lens = torch.zeros(1, dtype=torch.int32)
+    for k, v in ((x, None), (None, x)):
+        with pytest.raises(ValueError):
+            ops.flash_attn_with_kvcache8(x, cache, k, v, cache_seqlens=lens)
+    assert not cache.keys.view(torch.uint8).any() and not cache.key_scales.any()
+
+
 @pytest.mark.gpu
 def test_kernel_refusals():
     from myk_llm_b200 import ops
