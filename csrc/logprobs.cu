@@ -4,6 +4,7 @@
 //   with S = sum e^{x_j - m}, T = sum e^{x_j - m} (x_j - m)  (T <= 0: no cancellation)
 //   top k: largest logits, the lowest index first among equal ones
 //   dx_j = [j = t] g + sum_i [j = top_i] h_i - p_j (g + sum h + gH (log p_j + H))
+// A row without a logit above -inf has S = 0 (any other has S >= 1) and no distribution; a NaN or +inf makes S NaN.
 //
 // Both directions are bound by reading (and writing) the logits once.
 #include <torch/extension.h>
@@ -58,10 +59,15 @@ struct Stat {
   float m, s, t;
 };
 __device__ __forceinline__ float ref_of(float m) { return m == -INFINITY ? 0.f : m; }
+// m less the reference r >= m, kept finite for m = -inf, as e^-1000 is 0 already.  inf - inf stays NaN (a maximum
+// with -1000 would drop it), so a +inf among the logits shows in the sums wherever it lies in the row.
+__device__ __forceinline__ float shift_of(float m, float r) {
+  const float d = m - r;
+  return d < -1000.f ? -1000.f : d;
+}
 __device__ __forceinline__ Stat join(Stat a, Stat b) {
   const float m = fmaxf(a.m, b.m), r = ref_of(m);
-  // an empty side has s = t = 0 and m = -inf; shifts are kept finite, as e^-1000 is 0 already
-  const float da = fmaxf(a.m - r, -1000.f), db = fmaxf(b.m - r, -1000.f);
+  const float da = shift_of(a.m, r), db = shift_of(b.m, r);  // an empty side has s = t = 0 and m = -inf
   const float ea = exp2f(da * kLog2e), eb = exp2f(db * kLog2e);
   return {m, a.s * ea + b.s * eb, ea * (a.t + a.s * da) + eb * (b.t + b.s * db)};
 }
@@ -163,7 +169,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 5 : 1) fwd_kernel(Fw
     if (TOP && st < kSteps) step_max[st][tid] = mx;
     mine = fmaxf(mine, mx);
     const float m = fmaxf(a.m, mx), r = ref_of(m);
-    const float d = fmaxf(a.m - r, -1000.f), c = exp2f(d * kLog2e);
+    const float d = shift_of(a.m, r), c = exp2f(d * kLog2e);
     float2 s2 = make_float2(a.s * c, 0.f), t2 = make_float2(c * (a.t + a.s * d), 0.f);
     const float2 neg = make_float2(-r, -r), l2 = make_float2(kLog2e, kLog2e);
 #pragma unroll

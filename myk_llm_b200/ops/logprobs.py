@@ -10,7 +10,7 @@ the backward pass reads the logits once more and writes their gradient.
 A token equal to ``ignore_index`` gets log probability 0 and no gradient through it; one
 outside the vocabulary gets NaN.  Logits of -inf (excluded tokens) have probability 0.  A row
 that is -inf throughout has no distribution: log probabilities -inf, entropy 0, gradient 0.
-A NaN anywhere in a row makes its numbers NaN.
+A NaN or +inf anywhere in a row makes its numbers and its gradient NaN.
 """
 
 from __future__ import annotations

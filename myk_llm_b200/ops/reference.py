@@ -243,8 +243,9 @@ def token_logprobs_ref(logits, tokens, top, ignore_index=IGNORE_INDEX):
     vocab = x.shape[-1]
     empty = (x == -math.inf).all(-1)
     none = empty[..., None].expand_as(x)
-    lse = torch.logsumexp(torch.where(none, torch.zeros_like(x), x), -1, keepdim=True)
-    z = torch.where(none, torch.full_like(x, -math.inf), x - lse)
+    y = torch.where(none, torch.zeros_like(x), x)
+    y = y - y.detach().amax(-1, keepdim=True)  # a NaN or +inf makes the sum, and so the whole row, NaN
+    z = torch.where(none, torch.full_like(x, -math.inf), y - y.exp().sum(-1, keepdim=True).log())
     out_of_range = (tokens < 0) | (tokens >= vocab)
     lp = z.gather(-1, tokens.long().clamp(0, vocab - 1)[..., None])[..., 0]
     lp = torch.where(out_of_range, torch.full_like(lp, math.nan), lp)

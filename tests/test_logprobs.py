@@ -207,6 +207,57 @@ def test_special_rows_gpu():
     _special("cuda")
 
 
+def _infinite(device, dtype, vocab, lo):
+    """+inf wherever it lies in a row (first, in the middle, last; alone or beside -inf and NaN) makes the row's
+    numbers and gradient NaN and touches no other row; -inf throughout stays "no distribution"."""
+    from myk_llm_b200 import ops
+
+    top = min(3, vocab)
+    at = sorted({0, 1 % vocab, 7 % vocab, vocab // 2, vocab - 9 if vocab > 9 else 0, vocab - 2 if vocab > 1 else 0, vocab - 1})
+    rows = 2 * len(at) + 3
+    wide = torch.zeros(rows, vocab + lo + 5, dtype=dtype, device=device)
+    x = wide[:, lo:lo + vocab]
+    data, t = _logits(rows, vocab, "normal", dtype, device, seed=7)
+    x.copy_(data)
+    for i, j in enumerate(at):
+        x[i, j] = math.inf
+        x[len(at) + i] = -math.inf
+        x[len(at) + i, j] = math.inf
+    x[-1] = -math.inf
+    x[-2] = -math.inf
+    x[-2, vocab - 1] = math.nan
+    bad = torch.arange(rows, device=device) < 2 * len(at)
+    bad[-2] = True
+    sound = torch.tensor([rows - 3], device=device)
+    leaf = x.detach().requires_grad_()
+    r = ops.token_logprobs(leaf, t, top=top)
+    for y in r[:3]:
+        assert y[bad].isnan().all() and not y[~bad].isnan().any()
+    for i, j in enumerate(at):
+        assert r.top_tokens[i, 0] == j and r.top_tokens[len(at) + i, 0] == j
+    _check(x[sound], t[sound], top, [y.detach()[sound] for y in r])
+    assert r.logprobs[-1] == -math.inf and r.entropy[-1] == 0 and (r.top_logprobs[-1] == -math.inf).all()
+    for out in (r.logprobs, r.entropy, r.top_logprobs):
+        g, = torch.autograd.grad(out[:-1].sum(), leaf, retain_graph=True)
+        assert g[bad].isnan().all() and not g[~bad].isnan().any() and not g[-1].any()
+
+
+INFINITE = [(1, 0), (2, 1), (9, 0), (37, 3), (1000, 1), (4099, 0), (20011, 5)]  # (vocabulary, offset of the rows)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab,lo", INFINITE)
+def test_infinite_logits_cpu(vocab, lo, dtype):
+    _infinite("cpu", dtype, vocab, lo)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab,lo", INFINITE)
+def test_infinite_logits_gpu(vocab, lo, dtype):
+    _infinite("cuda", dtype, vocab, lo)
+
+
 def _differences(device):
     """The gradient along random directions against central differences in fp64."""
     from myk_llm_b200 import ops
