@@ -5,7 +5,8 @@ alternatives, from logits.
 copy of them.  Ties among the alternatives go to the lowest token id.  The log
 probabilities, the entropy and the alternatives' log probabilities are differentiable with
 respect to the logits (policy gradients, entropy bonuses, distillation onto the top tokens);
-the backward pass reads the logits once more and writes their gradient.
+the backward pass reads the logits once more and writes their gradient.  On CUDA there is no
+second derivative (asking for it raises).
 
 A token equal to ``ignore_index`` gets log probability 0 and no gradient through it; one
 outside the vocabulary gets NaN.  Logits of -inf (excluded tokens) have probability 0.  A row
@@ -47,7 +48,19 @@ class _TokenLogprobs(torch.autograd.Function):
         logits, tokens, lse, ent, tt = ctx.saved_tensors
         if g_lp is None and g_ent is None and g_top is None:
             return None, None, None, None
-        return ext().logprobs_bwd(logits, tokens, ctx.ignore_index, lse, ent, tt, g_lp, g_ent, g_top), None, None, None
+        return _Gradient.apply(logits, tokens, ctx.ignore_index, lse, ent, tt, g_lp, g_ent, g_top), None, None, None
+
+
+class _Gradient(torch.autograd.Function):
+    """The gradient, as a function of its own so that differentiating it again is an error."""
+
+    @staticmethod
+    def forward(ctx, *args):
+        return ext().logprobs_bwd(*args)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("token_logprobs has no second derivative on CUDA")
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0,

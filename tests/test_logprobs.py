@@ -293,6 +293,18 @@ def test_gradient_differences_gpu():
 
 
 @pytest.mark.gpu
+def test_second_derivative_is_refused():
+    """The kernels have a first derivative; differentiating it again is an error, not a wrong gradient."""
+    from myk_llm_b200 import ops
+
+    x, t = _logits(5, 101, "normal", torch.float32, "cuda")
+    leaf = x.clone().requires_grad_()
+    g, = torch.autograd.grad(ops.token_logprobs(leaf, t).logprobs.sum(), leaf, create_graph=True)
+    with pytest.raises(RuntimeError):
+        (g.square().sum() + 0.0 * leaf.sum()).backward()
+
+
+@pytest.mark.gpu
 def test_shapes_strides_and_partial_gradients():
     """Batched shapes, padded vocabularies (rows apart, unaligned), transposed logits, int32
     tokens, another stream, and gradients through one output alone."""
