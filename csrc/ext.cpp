@@ -140,8 +140,8 @@ torch::Tensor kv8_attend(torch::Tensor q, torch::Tensor keys, torch::Tensor valu
                          int64_t right);
 // logprobs.cu
 std::vector<torch::Tensor> logprobs_fwd(torch::Tensor logits, torch::Tensor tokens, int64_t top, int64_t ignore);
-torch::Tensor logprobs_bwd(torch::Tensor logits, torch::Tensor tokens, int64_t ignore, torch::Tensor lse,
-                           torch::Tensor entropy, torch::Tensor top_tok, c10::optional<torch::Tensor> g_lp,
+torch::Tensor logprobs_bwd(torch::Tensor logits, torch::Tensor tokens, int64_t ignore, torch::Tensor stats,
+                           torch::Tensor top_tok, c10::optional<torch::Tensor> g_lp,
                            c10::optional<torch::Tensor> g_ent, c10::optional<torch::Tensor> g_top);
 }  // namespace mykb
 

@@ -88,8 +88,10 @@ struct FwdParams {
   int64_t stride;  // elements between rows
   const int64_t* tokens;
   int64_t ignore;
-  float *logprob, *entropy, *lse, *top_lp;
+  float *logprob, *entropy, *top_lp;
+  float* stats;  // (2, rows) for the gradient: lse, entropy
   int64_t* top_tok;
+  int64_t rows;
   int V, top;
 };
 
@@ -206,8 +208,9 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 5 : 1) fwd_kernel(Fw
       else out = all.s == 0.f ? -INFINITY : Vec<T>::load(x + t) - lse;
     }
     p.logprob[row] = out;
-    p.entropy[row] = all.s == 0.f ? 0.f : __logf(all.s) - all.t / all.s;
-    p.lse[row] = lse;
+    const float entropy = all.s == 0.f ? 0.f : __logf(all.s) - all.t / all.s;
+    p.entropy[row] = entropy;
+    p.stats[row] = lse, p.stats[p.rows + row] = entropy;
   }
   if constexpr (TOP) {
     __shared__ uint32_t lists[WARPS][32];
@@ -335,9 +338,10 @@ struct BwdParams {
   int64_t stride;
   const int64_t* tokens;
   int64_t ignore;
-  const float *lse, *entropy;
+  const float* stats;  // (2, rows): lse, entropy
   const float *g_lp, *g_ent, *g_top;  // any may be null
   const int64_t* top_tok;
+  int64_t rows;
   int V, top, chunk, chunks;
 };
 
@@ -353,14 +357,14 @@ __global__ void __launch_bounds__(THREADS) bwd_kernel(BwdParams<T> p) {
   const T* x = p.x + row * p.stride;
   T* dx = p.dx + row * p.V;
   const int64_t t = p.tokens[row];
-  const bool empty = p.lse[row] == -INFINITY;  // no distribution: no gradient
+  const bool empty = p.stats[row] == -INFINITY;  // no distribution: no gradient
   const bool given = p.g_lp && t != p.ignore && t >= 0 && t < p.V && !empty;
   const float gl = given ? p.g_lp[row] : 0.f, gh = p.g_ent && !empty ? p.g_ent[row] : 0.f;
   float A = gl;
   if (p.g_top && !empty)
     for (int i = 0; i < p.top; ++i) A += p.g_top[row * p.top + i];
-  const float lse = empty ? 0.f : p.lse[row];
-  A = fmaf(gh, p.entropy[row], A);  // g = -p (A + gh log p)
+  const float lse = empty ? 0.f : p.stats[row];
+  A = fmaf(gh, p.stats[p.rows + row], A);  // g = -p (A + gh log p)
   const float nA = -A, ngh = -gh;
   auto dense = [&](float v) {
     const float z = v - lse;
@@ -428,17 +432,18 @@ static void check(const torch::Tensor& logits, const torch::Tensor& tokens, int6
 
 }  // namespace lp
 
-// (logprob, entropy, lse, top_logprob, top_token) of each row.
+// (logprob, entropy, what the gradient needs, top_logprob, top_token) of each row, each a tensor of its own:
+// a user may change the outputs in place before the gradient is taken.
 std::vector<torch::Tensor> logprobs_fwd(torch::Tensor logits, torch::Tensor tokens, int64_t top, int64_t ignore) {
   using namespace lp;
   check(logits, tokens, top, "token_logprobs");
   c10::cuda::CUDAGuard guard(logits.device());
   const int64_t rows = logits.size(0);
   auto f = logits.options().dtype(at::kFloat);
-  auto stats = torch::empty({3, rows}, f);
+  auto lp = torch::empty({rows}, f), ent = torch::empty({rows}, f), stats = torch::empty({2, rows}, f);
   auto tl = torch::empty({rows, top}, f);
   auto tt = torch::empty({rows, top}, tokens.options());
-  std::vector<torch::Tensor> out{stats[0], stats[1], stats[2], tl, tt};
+  std::vector<torch::Tensor> out{lp, ent, stats, tl, tt};
   if (rows == 0) return out;
   cudaStream_t st = at::cuda::getCurrentCUDAStream();
   auto go = [&](auto* ptr) {
@@ -447,7 +452,8 @@ std::vector<torch::Tensor> logprobs_fwd(torch::Tensor logits, torch::Tensor toke
     p.x = ptr;
     p.stride = logits.stride(0);
     p.tokens = tokens.data_ptr<int64_t>(), p.ignore = ignore;
-    p.logprob = stats.data_ptr<float>(), p.entropy = p.logprob + rows, p.lse = p.entropy + rows;
+    p.logprob = lp.data_ptr<float>(), p.entropy = ent.data_ptr<float>(), p.stats = stats.data_ptr<float>();
+    p.rows = rows;
     p.top_lp = tl.data_ptr<float>(), p.top_tok = tt.data_ptr<int64_t>();
     p.V = (int)logits.size(1), p.top = (int)top;
     // few rows: latency counts, a row's loads are spread over four times the threads (8 rows of 65536 bf16
@@ -467,8 +473,8 @@ std::vector<torch::Tensor> logprobs_fwd(torch::Tensor logits, torch::Tensor toke
   return out;
 }
 
-torch::Tensor logprobs_bwd(torch::Tensor logits, torch::Tensor tokens, int64_t ignore, torch::Tensor lse,
-                           torch::Tensor entropy, torch::Tensor top_tok, c10::optional<torch::Tensor> g_lp,
+torch::Tensor logprobs_bwd(torch::Tensor logits, torch::Tensor tokens, int64_t ignore, torch::Tensor stats,
+                           torch::Tensor top_tok, c10::optional<torch::Tensor> g_lp,
                            c10::optional<torch::Tensor> g_ent, c10::optional<torch::Tensor> g_top) {
   using namespace lp;
   check(logits, tokens, top_tok.size(1), "token_logprobs backward");
@@ -490,7 +496,7 @@ torch::Tensor logprobs_bwd(torch::Tensor logits, torch::Tensor tokens, int64_t i
     p.x = ptr, p.dx = (T*)dx.data_ptr();
     p.stride = logits.stride(0);
     p.tokens = tokens.data_ptr<int64_t>(), p.ignore = ignore;
-    p.lse = lse.data_ptr<float>(), p.entropy = entropy.data_ptr<float>();
+    p.stats = stats.data_ptr<float>(), p.rows = rows;
     p.top = (int)top_tok.size(1), p.top_tok = top_tok.data_ptr<int64_t>();
     p.g_lp = grad(g_lp, rows), p.g_ent = grad(g_ent, rows), p.g_top = grad(g_top, rows * p.top);
     p.V = (int)V;

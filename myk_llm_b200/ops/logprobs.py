@@ -36,8 +36,8 @@ class TokenLogprobs(NamedTuple):
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, top, ignore_index):
-        lp, ent, lse, tl, tt = ext().logprobs_fwd(logits, tokens, top, ignore_index)
-        ctx.save_for_backward(logits, tokens, lse, ent, tt)
+        lp, ent, stats, tl, tt = ext().logprobs_fwd(logits, tokens, top, ignore_index)
+        ctx.save_for_backward(logits, tokens, stats, tt)
         ctx.ignore_index = ignore_index
         ctx.mark_non_differentiable(tt)
         ctx.set_materialize_grads(False)
@@ -45,10 +45,10 @@ class _TokenLogprobs(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, g_lp, g_ent, g_top, _):
-        logits, tokens, lse, ent, tt = ctx.saved_tensors
+        logits, tokens, stats, tt = ctx.saved_tensors
         if g_lp is None and g_ent is None and g_top is None:
             return None, None, None, None
-        return _Gradient.apply(logits, tokens, ctx.ignore_index, lse, ent, tt, g_lp, g_ent, g_top), None, None, None
+        return _Gradient.apply(logits, tokens, ctx.ignore_index, stats, tt, g_lp, g_ent, g_top), None, None, None
 
 
 class _Gradient(torch.autograd.Function):

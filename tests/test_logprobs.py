@@ -292,6 +292,41 @@ def test_gradient_differences_gpu():
     _differences("cuda")
 
 
+def _in_place(device):
+    """Outputs masked in place before backward: the gradient of the masked values."""
+    from myk_llm_b200 import ops
+
+    x, t = _logits(12, 503, "normal", torch.float32, device)
+    pad = torch.arange(12, device=device) % 3 == 0
+    for shape in ((12,), (3, 4)):
+        grads = []
+        for in_place in (False, True):
+            leaf = x.clone().requires_grad_()
+            r = ops.token_logprobs(leaf.view(*shape, 503), t.view(shape), top=4)
+            lp, ent, tl = r.logprobs, r.entropy, r.top_logprobs
+            mask = pad.view(shape)
+            if in_place:
+                lp.masked_fill_(mask, 0.0)
+                lp.mul_(2.0)
+                ent[mask] = 0.0
+                tl.clamp_(min=-4.0)
+            else:
+                lp = 2.0 * lp.masked_fill(mask, 0.0)
+                ent = ent.masked_fill(mask, 0.0)
+                tl = tl.clamp(min=-4.0)
+            grads.append(torch.autograd.grad(lp.sum() + 0.1 * ent.sum() + tl.sum(), leaf)[0])
+        assert torch.equal(*grads)
+
+
+def test_outputs_in_place_cpu():
+    _in_place("cpu")
+
+
+@pytest.mark.gpu
+def test_outputs_in_place_gpu():
+    _in_place("cuda")
+
+
 @pytest.mark.gpu
 def test_second_derivative_is_refused():
     """The kernels have a first derivative; differentiating it again is an error, not a wrong gradient."""
