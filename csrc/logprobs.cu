@@ -1,7 +1,8 @@
 // Log probabilities of given tokens with entropy and top alternatives, and their gradient.
 //
-//   lse = log sum_j e^{x_j},  logprob = x_t - lse,  H = -sum_j p_j log p_j = log S - T / S
-//   with S = sum e^{x_j - m}, T = sum e^{x_j - m} (x_j - m)  (T <= 0: no cancellation)
+//   logprob = (x_t - m) - log S,  H = -sum_j p_j log p_j = log S - T / S
+//   with m = max x_j, S = sum e^{x_j - m}, T = sum e^{x_j - m} (x_j - m)  (T <= 0: no cancellation)
+//   (not x_t - (m + log S), which would round log S at the size of the logits)
 //   top k: largest logits, the lowest index first among equal ones
 //   dx_j = [j = t] g + sum_i [j = top_i] h_i - p_j (g + sum h + gH (log p_j + H))
 // A row without a logit above -inf has S = 0 (any other has S >= 1) and no distribution; a NaN or +inf makes S NaN.
@@ -89,7 +90,7 @@ struct FwdParams {
   const int64_t* tokens;
   int64_t ignore;
   float *logprob, *entropy, *top_lp;
-  float* stats;  // (2, rows) for the gradient: lse, entropy
+  float* stats;  // (3, rows) for the gradient: m, log S, entropy
   int64_t* top_tok;
   int64_t rows;
   int V, top;
@@ -199,18 +200,18 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 5 : 1) fwd_kernel(Fw
   Stat all = red[0];
 #pragma unroll
   for (int w = 1; w < WARPS; ++w) all = join(all, red[w]);
-  const float lse = all.s == 0.f ? -INFINITY : all.m + __logf(all.s);
+  const float logs = __logf(all.s);  // -inf for a row without a distribution
   if (tid == 0) {
     const int64_t t = p.tokens[row];
     float out = 0.f;
     if (t != p.ignore) {
       if (t < 0 || t >= V) out = __int_as_float(0x7fffffff);  // not a token of this vocabulary: NaN
-      else out = all.s == 0.f ? -INFINITY : Vec<T>::load(x + t) - lse;
+      else out = all.s == 0.f ? -INFINITY : (Vec<T>::load(x + t) - all.m) - logs;
     }
     p.logprob[row] = out;
-    const float entropy = all.s == 0.f ? 0.f : __logf(all.s) - all.t / all.s;
+    const float entropy = all.s == 0.f ? 0.f : logs - all.t / all.s;
     p.entropy[row] = entropy;
-    p.stats[row] = lse, p.stats[p.rows + row] = entropy;
+    p.stats[row] = all.m, p.stats[p.rows + row] = logs, p.stats[2 * p.rows + row] = entropy;
   }
   if constexpr (TOP) {
     __shared__ uint32_t lists[WARPS][32];
@@ -324,7 +325,7 @@ __global__ void __launch_bounds__(THREADS, THREADS == 256 ? 5 : 1) fwd_kernel(Fw
       int rank = 0;
       for (int j = 0; j < n; ++j) rank += cand[j] > c;
       if (rank < k) {
-        p.top_lp[row * k + rank] = all.s == 0.f ? -INFINITY : value_of((uint32_t)(c >> 32)) - lse;
+        p.top_lp[row * k + rank] = all.s == 0.f ? -INFINITY : (value_of((uint32_t)(c >> 32)) - all.m) - logs;
         p.top_tok[row * k + rank] = (int64_t)(uint32_t)~(uint32_t)c;
       }
     }
@@ -338,7 +339,7 @@ struct BwdParams {
   int64_t stride;
   const int64_t* tokens;
   int64_t ignore;
-  const float* stats;  // (2, rows): lse, entropy
+  const float* stats;  // (3, rows): m, log S, entropy
   const float *g_lp, *g_ent, *g_top;  // any may be null
   const int64_t* top_tok;
   int64_t rows;
@@ -357,17 +358,17 @@ __global__ void __launch_bounds__(THREADS) bwd_kernel(BwdParams<T> p) {
   const T* x = p.x + row * p.stride;
   T* dx = p.dx + row * p.V;
   const int64_t t = p.tokens[row];
-  const bool empty = p.stats[row] == -INFINITY;  // no distribution: no gradient
+  const bool empty = p.stats[p.rows + row] == -INFINITY;  // no distribution: no gradient
   const bool given = p.g_lp && t != p.ignore && t >= 0 && t < p.V && !empty;
   const float gl = given ? p.g_lp[row] : 0.f, gh = p.g_ent && !empty ? p.g_ent[row] : 0.f;
   float A = gl;
   if (p.g_top && !empty)
     for (int i = 0; i < p.top; ++i) A += p.g_top[row * p.top + i];
-  const float lse = empty ? 0.f : p.stats[row];
-  A = fmaf(gh, p.stats[p.rows + row], A);  // g = -p (A + gh log p)
+  const float m = empty ? 0.f : p.stats[row], logs = empty ? 0.f : p.stats[p.rows + row];
+  A = fmaf(gh, p.stats[2 * p.rows + row], A);  // g = -p (A + gh log p)
   const float nA = -A, ngh = -gh;
   auto dense = [&](float v) {
-    const float z = v - lse;
+    const float z = (v - m) - logs;
     float e, g;  // without flushing: a subnormal p may meet a large factor
     asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(z * kLog2e));
     asm("mul.rn.f32 %0, %1, %2;" : "=f"(g) : "f"(e), "f"(fmaf(ngh, fmaxf(z, -1000.f), nA)));
@@ -440,7 +441,7 @@ std::vector<torch::Tensor> logprobs_fwd(torch::Tensor logits, torch::Tensor toke
   c10::cuda::CUDAGuard guard(logits.device());
   const int64_t rows = logits.size(0);
   auto f = logits.options().dtype(at::kFloat);
-  auto lp = torch::empty({rows}, f), ent = torch::empty({rows}, f), stats = torch::empty({2, rows}, f);
+  auto lp = torch::empty({rows}, f), ent = torch::empty({rows}, f), stats = torch::empty({3, rows}, f);
   auto tl = torch::empty({rows, top}, f);
   auto tt = torch::empty({rows, top}, tokens.options());
   std::vector<torch::Tensor> out{lp, ent, stats, tl, tt};

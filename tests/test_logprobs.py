@@ -258,6 +258,38 @@ def test_infinite_logits_gpu(vocab, lo, dtype):
     _infinite("cuda", dtype, vocab, lo)
 
 
+def _shifted(device, vocab, shift):
+    """Logits far from 0.  They are multiples of 2^-3 below 2^20, so differences to the maximum are exact in fp32 and a
+    shift changes no result: a log probability (x_t - m) - log S may be off by 2^-20 (1 + |logprob|), the entropy by
+    2^-19 (1 + H), whatever the size of the logits, and the gradient as everywhere in this file."""
+    from myk_llm_b200 import ops
+
+    rows, top = 5, min(6, vocab)
+    g = torch.Generator(device=device).manual_seed(3)
+    x = torch.randint(-80, 81, (rows, vocab), generator=g, device=device) * 0.125 + shift
+    t = torch.randint(0, vocab, (rows,), generator=g, device=device)
+    r = ops.token_logprobs(x, t, top=top)
+    wl, we, wtl, order, *_ = _exact(x - shift, t, top)
+    assert torch.equal(r.top_tokens, order)
+    for got, want, tol in ((r.logprobs, wl, 2.0 ** -20), (r.entropy, we, 2.0 ** -19), (r.top_logprobs, wtl, 2.0 ** -20)):
+        assert bool(((got.double() - want).abs() <= tol * (1 + want.abs())).all())
+    _check_grad(x, t, top, device)
+
+
+SHIFTED = [(v, s) for v in (3, 1000, 40001) for s in (0.0, 2.0 ** 17, -(2.0 ** 19))]
+
+
+@pytest.mark.parametrize("vocab,shift", SHIFTED)
+def test_shifted_logits_cpu(vocab, shift):
+    _shifted("cpu", vocab, shift)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab,shift", SHIFTED)
+def test_shifted_logits_gpu(vocab, shift):
+    _shifted("cuda", vocab, shift)
+
+
 def _differences(device):
     """The gradient along random directions against central differences in fp64."""
     from myk_llm_b200 import ops
