@@ -817,6 +817,15 @@ static void launch_fwd(const CUtensorMap& tq, const CUtensorMap& tk, const CUten
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
+// Work items that launch_fwd's busiest CTA takes in turn for a batch of `seqs` x `max_q` queries (places of a band that
+// hold no tile count: they fall to the same CTAs in every band).
+int64_t fa_fwd_rounds(int head_dim, int heads, int kv_heads, int64_t seqs, int64_t max_q, int sms) {
+  const bool pairs = heads / kv_heads % 2 == 0;
+  const int64_t tiles = (max_q + 127) / 128, cols = seqs * (pairs ? heads / 2 : heads);
+  const int64_t ctas = (int64_t)sms * (head_dim == 64 && !pairs ? 2 : 1);
+  return ((tiles + kBand - 1) / kBand * kBand * cols + ctas - 1) / ctas;
+}
+
 std::vector<torch::Tensor> fa_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, c10::optional<torch::Tensor> cu_q,
                                   c10::optional<torch::Tensor> cu_k, c10::optional<torch::Tensor> seqused_k,
                                   int64_t max_q, int64_t max_k, double scale, int64_t left, int64_t right) {

@@ -42,6 +42,7 @@ namespace mykb {
 std::vector<torch::Tensor> fa_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, c10::optional<torch::Tensor> cu_q,
                                   c10::optional<torch::Tensor> cu_k, c10::optional<torch::Tensor> seqused_k,
                                   int64_t max_q, int64_t max_k, double scale, int64_t left, int64_t right);
+int64_t fa_fwd_rounds(int head_dim, int heads, int kv_heads, int64_t seqs, int64_t max_q, int sms);
 namespace kv8 {
 
 constexpr int WARPS = 4;
@@ -637,17 +638,26 @@ __global__ void __launch_bounds__(THREADS) join_kernel(AttendParams p) {
       make_uint2(pack_bf16x2(a.x * inv, a.y * inv), pack_bf16x2(a.z * inv, a.w * inv));
 }
 
-// Whether to read the cache back to bf16 and run the prefill kernel instead.  attend_kernel takes
-// about 0.05 ns a key and column (0.037 at head_dim 64: its tiles come from L2 after the first row
-// tile); the prefill kernel 20 ns a key for each wave of its (128 queries, head) items over the
-// SMs, which is all it is split over, plus the read back at HBM speed.  Measured, us: 1 x 512
-// queries, 16/4 heads of 128, 2048 keys: 72 here, 48 there; 4 x 509, 4096 keys: 384, 88; 8 x 32,
-// 8192 keys: 100, 313; 13 x 155 queries of one head, 30000 keys: 162, 627; 64 x 64, 16/4 heads of
-// 64, 2048 keys: 298, 507.  Up to 64 rows a KV head always stay here.
-static bool prefer_prefill(const Cache& c, int H, int L, int64_t columns, int64_t span, int sms) {
-  const double here = (c.D == 64 ? 0.037 : 0.05) * columns * span;
-  const int64_t items = (int64_t)c.B * H * ((L + 127) / 128);
-  const double there = 20.0 * ((items + sms - 1) / sms) * span + 0.0016 * c.D * c.B * c.Hkv * c.cap;
+// Whether to read the cache back to bf16 and run the prefill kernel instead, by what both take in ns.
+// Here: 18 a column (its 16 rows are joined by as many CTAs) and 0.04 a key and column (0.028 at head_dim 64: its
+// tiles come from L2 after the first row tile).  There: the keys of the items that one CTA of the prefill kernel takes
+// in turn, which is all it is split over, at 17 a key where an item is two heads (even groups) and 20 where it is one,
+// plus the read back of the whole capacity at HBM speed.  The lengths are known on the device only, so both sides
+// stand for full sequences.
+// Measured here / there, us (predicted in brackets): 4 x 509 queries, 16/4 heads of 128, ragged to 4096 keys:
+// 173 / 56 (384 / 92); 1 x 512, 16/4 of 64, 2048: 57 / 44 (50 / 49); 8 x 32, 16/4 of 128, 8192: 101 / 320 (100 / 326);
+// 13 x 155 of one head of 128, 30000: 162 / 633 (169 / 664); 64 x 64, 16/4 of 64, 2048: 296 / 509 (320 / 536);
+// 16 x 80, 16/4 of 64, ragged to 16000: 284 / 656 (608 / 1168); 6 x 184, 16/8 of 64, 966, window 512: 70 / 38 (53 / 39).
+// The faster side was taken for 59 of the 60 shapes that the figures were fitted to (the other cost 1.19 times the best)
+// and for 60 of 60 further ones (1 to 30 sequences, 22 to 2046 queries, 262 to 56913 keys, groups of 1 to 8).
+// Up to 64 rows a KV head always stay here.
+static bool prefer_prefill(const Cache& c, int H, int L, int64_t columns, int64_t span, int64_t left, int64_t right,
+                           int sms) {
+  const double here = 11e3 + columns * (18 + (c.D == 64 ? 0.028 : 0.04) * span);
+  // keys that 128 queries see
+  const int64_t keys = left >= 0 && right >= 0 ? std::min<int64_t>(c.cap, left + right + 128) : c.cap;
+  const double there = 14e3 + (H / c.Hkv % 2 == 0 ? 17.0 : 20.0) * fa_fwd_rounds(c.D, H, c.Hkv, c.B, L, sms) * keys +
+                       0.001 * c.D * c.B * c.Hkv * c.cap;
   return (int64_t)(H / c.Hkv) * L > 64 && (there < here || columns * ((c.cap + KT - 1) / KT) > INT32_MAX);
 }
 
@@ -692,7 +702,7 @@ torch::Tensor kv8_attend(torch::Tensor q, torch::Tensor keys, torch::Tensor valu
   int64_t span = c.cap;  // most keys a sequence can show
   if (left >= 0) span = std::min<int64_t>(span, left + L + KT);
   const int64_t columns = (int64_t)c.B * c.Hkv * RT;
-  if (prefer_prefill(c, H, L, columns, span, sms[c.device])) {
+  if (prefer_prefill(c, H, L, columns, span, left, right, sms[c.device])) {
     auto opt = q.options();
     auto kb = torch::empty({c.B, c.cap, c.Hkv, c.D}, opt), vb = torch::empty({c.B, c.cap, c.Hkv, c.D}, opt);
     read(c, lens, extra, nullptr, 0, c.cap, 256, kb, vb, who);  // 256: more than a key tile of the prefill kernel

@@ -616,6 +616,29 @@ def test_bad_queries_gpu():
     _bad_queries("cuda")
 
 
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [
+    # (batch, new, heads, kv_heads, d, cached keys, window, whether the prefill kernel is the faster one)
+    (16, 80, 16, 4, 64, 16000, 0, False),   # a wave of the prefill kernel's CTAs is mostly idle with one query tile
+    (16, 184, 16, 8, 64, 4000, 512, True),  # items of two heads, and a window that bounds the keys of each
+])
+def test_prefill_rule(case):
+    """Which kernel a call takes, by whether it holds a bf16 copy of the cache while it runs."""
+    from myk_llm_b200 import ops
+
+    b, new, heads, hk, d, cap, window, prefill = case
+    cache = ops.kv8_cache(b, cap, hk, d, device="cuda")
+    q = torch.zeros(b, new, heads, d, dtype=torch.bfloat16, device="cuda")
+    lens = torch.full((b,), cap // 2, dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    ops.flash_attn_with_kvcache8(q, cache, cache_seqlens=lens, causal=True, window_size=(window - 1, 0))
+    copy = 2 * 2 * b * cap * hk * d
+    assert (torch.cuda.max_memory_allocated() - before >= copy) == prefill
+
+
 # ------------------------------------------------------------------------- refusals
 def test_cache_refusals():
     from myk_llm_b200 import ops
