@@ -639,6 +639,31 @@ def test_prefill_rule(case):
     assert (torch.cuda.max_memory_allocated() - before >= copy) == prefill
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+@pytest.mark.parametrize("case", [c for c in ATTEND if c[3] // c[4] * c[1] > 64])
+def test_attend_split_weights(case, dtype):
+    """More than 64 rows a KV head over few keys: the split kernel, whose weights have f16's 11 bits (2^-10 sum p |v|)."""
+    from myk_llm_b200 import ops
+
+    lens, new, step, heads, hk, d, block, causal, window = case
+    assert causal and step
+    b, cap = len(lens), max(lens) + new + 5
+    cache, plain = _cache(b, cap, hk, d, dtype, block, "cuda")
+    held = [_data((b, cap, hk, d), s, "cuda", spread=False) for s in (1, 2)]
+    kv = [_data((b, new, hk, d), s, "cuda", spread=False) for s in (4, 5)]
+    zero = torch.zeros(b, dtype=torch.int32, device="cuda")
+    ops.kv8_append(cache, *held, cache_seqlens=zero)
+    q = _data((b, new, heads, d), 3, "cuda") * 0.5
+    out = ops.flash_attn_with_kvcache8(q, cache, *kv, cache_seqlens=zero + torch.tensor(lens, device="cuda"), causal=True,
+                                       window_size=window)
+    for p, x, y in zip(plain, held, kv):
+        p.append(x, [0] * b)
+        p.append(y, lens)
+    want, mag = _attend(q, plain[0].values(), plain[1].values(), [n + new for n in lens], window[0], 0, 1 / math.sqrt(d))
+    assert bool(((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * mag).all())
+
+
 # ------------------------------------------------------------------------- refusals
 def test_cache_refusals():
     from myk_llm_b200 import ops
