@@ -94,9 +94,17 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 // (both do nothing where the kernel was launched without that attribute).
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;"); }
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-// A tile has landed.  If it does not within a second, the status word says so and the kernel winds down.
-__device__ __forceinline__ void tile_wait(uint64_t* bar, uint32_t parity, int* status) {
-  if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) mbar_wait_warp(bar, parity, status, __LINE__);
+// Whether a tile has landed.  If it does not within a second, the status word says so.
+__device__ __forceinline__ bool tile_wait(uint64_t* bar, uint32_t parity, int* status) {
+  return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || mbar_wait_warp(bar, parity, status, __LINE__);
+}
+// For a warp that gives up: up to a second more for a copy in flight, whatever the status word says, as its shared
+// memory is another CTA's after the return.
+__device__ __noinline__ void tile_drain(uint64_t* bar, uint32_t parity) {
+  const uint64_t t0 = globaltimer_ns();
+  while (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity)) &&
+         !__any_sync(0xffffffffu, globaltimer_ns() - t0 > kWaitNs)) {
+  }
 }
 // Weight of a partial (m, l) when joined under the maximum M: 0 without any weight; a sum that is
 // not a number stays one.
@@ -355,7 +363,10 @@ attend_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ C
       for (int x = 0; x < NS; ++x) kx[x] = kbyte[x], vx[x] = vbyte[x];
       if (i + 1 < n) load_scales(i + 1);
       const uint32_t st = used % STAGES;
-      tile_wait(&full[warp][st], (used / STAGES) & 1, p.status);
+      if (!tile_wait(&full[warp][st], (used / STAGES) & 1, p.status)) {
+        for (; used != issued; ++used) tile_drain(&full[warp][used % STAGES], (used / STAGES) & 1);
+        return;
+      }
       ++used;
       const unsigned char* buf = slots + st * S::TILE;
       const int key0 = key_first + i * KT;
