@@ -127,7 +127,7 @@ def kv8_append_ref(data, scales, block, x, seqlens):
     for b, n in enumerate(seqlens.tolist()):
         n = max(n, 0)
         end = min(n + x.shape[1], data.shape[2])
-        for blk in range(n // block, -(-end // block)):
+        for blk in range(n // block, -(-end // block) if end > n else 0):
             first = blk * block
             lo, hi = max(n, first), min(end, first + block)
             rows = x[b, lo - n:hi - n].transpose(0, 1).float()  # (H, rows, D)

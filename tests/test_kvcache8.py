@@ -200,6 +200,36 @@ def test_append_special_values_gpu(dtype):
     _special("cuda", dtype)
 
 
+def _full(device, dtype):
+    """Tokens at and past the capacity are dropped, also where the last block is a partial one; the rest is untouched."""
+    from myk_llm_b200 import ops
+
+    for cap, block in ((40, 16), (8, 16), (33, 32), (20, 1), (64, 16)):
+        b, h, d = 5, 2, 64
+        lens = [cap, cap + 1, cap + 100, cap - 2, 0]
+        cache, plain = _cache(b, cap, h, d, dtype, block, device)
+        first = [_data((b, cap, h, d), s, device) for s in (1, 2)]
+        more = [_data((b, 7, h, d), s, device) * 64 for s in (3, 4)]  # would raise every scale
+        zero = torch.zeros(b, dtype=torch.int32, device=device)
+        ops.kv8_append(cache, *first, cache_seqlens=zero)
+        ops.kv8_append(cache, *more, cache_seqlens=torch.tensor(lens, dtype=torch.int32, device=device))
+        for got, p, x, y in zip(ops.kv8_read(cache, cache_seqlens=zero + cap), plain, first, more):
+            p.append(x, [0] * b)
+            p.append(y, lens)
+            assert torch.equal(got.double(), _read(p, [cap] * b, [0] * b, cap))
+
+
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+def test_append_past_the_capacity_cpu(dtype):
+    _full("cpu", dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [E4M3, INT8])
+def test_append_past_the_capacity_gpu(dtype):
+    _full("cuda", dtype)
+
+
 @pytest.mark.gpu
 def test_append_strided_and_split_calls():
     """New tokens as slices of a fused projection (rows apart, some not 16-byte aligned) and,
