@@ -24,12 +24,16 @@
 // that do not depend on timing.
 //
 // Measured (B200, CUDA graph, both kernels): 64 sequences of 8192 tokens, 16/4 heads of 128, e4m3:
-// 95.5 us, 0.86 of the copy bandwidth (per-lane asynchronous copies instead of TMA: 117 us, of
-// which the loads alone took 116).  Two sequences of 131071 tokens: 59.5 us, 0.69 (the join of 222
+// 96.5 us, 0.85 of the copy bandwidth (per-lane asynchronous copies instead of TMA: 117 us, of
+// which the loads alone took 116).  Two sequences of 131071 tokens: 59.7 us, 0.69 (the join of 222
 // partials a column is 10 us of it).  Small calls are bound by latency: one sequence of 2048
-// tokens 9.2 us, 48 sequences that see 512 tokens 11.6 us.  Three queries a sequence (two MMA
+// tokens 9.1 us, 48 sequences that see 512 tokens 11.5 us.  Three queries a sequence (two MMA
 // columns a row tile, 12 warps an SM): bound by the chain QK -> exp -> PV of each warp's few
 // tiles, 64 ragged sequences of up to 2048 tokens 28 us for 31 MB.
+//
+// Wide calls (prefer_prefill) read the cache back to bf16 and run the bf16 prefill kernel, whose
+// weights have bf16's 8 bits instead of 11: 4 x 509 queries behind up to 4096 keys are 0.0022 off
+// the result in 64 bits, relative to its norm, of which the rounding of the output is 0.0017.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>

@@ -1,8 +1,9 @@
 // Writing and reading the 8-bit key/value cache (formats and scales: kv8.cuh).
 //
-// Both are one pass over their data, bound by HBM and, for a decode step's few tokens, by launch
-// latency.  8 x 2048 tokens of 4 heads of 128 (B200): written 13.5 us (50 MB), read back 12.3 us
-// (50 MB), each timed alone with a cold L2; one token for each of 8 sequences 4.7 us.
+// Both are one pass over their data, bound by the loads that short-lived CTAs keep in flight and, for
+// a decode step's few tokens, by launch latency.  8 x 2048 tokens of 4 heads of 128 (B200): written
+// 13.5 us (50 MB, 0.57 of the copy bandwidth), read back 12.3 us (50 MB, 0.63), each timed alone
+// with a cold L2; one token for each of 8 sequences 4.7 us.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>

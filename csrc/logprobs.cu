@@ -116,9 +116,10 @@ __device__ __forceinline__ uint32_t warp_merge(uint32_t v, int lane) {  // of a 
 }
 
 // One CTA a row, one pass over it: 4096 rows of 65536 bf16 logits with 5 alternatives take 127 us
-// (0.65 of the copy bandwidth; two vectors a thread ahead and five CTAs an SM were the best of the
-// depths and occupancies tried, 127 to 208 us), bound by the exponentials and the joins at the
-// ends of rows as much as by the loads.  The row's top k are found from the threads' own maxima: the
+// (0.64 of the copy bandwidth; two vectors a thread ahead and five CTAs an SM were the best of the
+// depths and occupancies tried, 127 to 208 us).  Bound by latency: loads stop at the joins and the
+// ranking at every row's end (long scoreboard and barrier are the stalls; no pipe is above 40 percent,
+// the one of the exponentials at 39).  The row's top k are found from the threads' own maxima: the
 // k-th largest of those is at most the k-th largest logit, so only the few elements that reach
 // it are candidates; threads that have one read those steps of theirs again (from L2), and the
 // candidates are ranked by counting.  Rows with so many equal logits that the candidates do not
@@ -346,8 +347,8 @@ struct BwdParams {
   int V, top, chunk, chunks;
 };
 
-// One CTA per (row, run of `chunk` logits), bound by HBM (4095 rows of 32768 bf16 logits: 94 us for
-// 537 MB, 0.87 of the copy bandwidth): the dense part, then the given and top tokens of the
+// One CTA per (row, run of `chunk` logits), bound by HBM (4095 rows of 32768 bf16 logits: 88 us for
+// 537 MB, 0.93 of the copy bandwidth; rows that are not 16-byte aligned go element by element): the dense part, then the given and top tokens of the
 // run are written again with their own terms.
 template <typename T>
 __global__ void __launch_bounds__(THREADS) bwd_kernel(BwdParams<T> p) {
@@ -457,8 +458,11 @@ std::vector<torch::Tensor> logprobs_fwd(torch::Tensor logits, torch::Tensor toke
     p.rows = rows;
     p.top_lp = tl.data_ptr<float>(), p.top_tok = tt.data_ptr<int64_t>();
     p.V = (int)logits.size(1), p.top = (int)top;
-    // few rows: latency counts, a row's loads are spread over four times the threads (8 rows of 65536 bf16
-    // logits: 13 us instead of 15); many rows: several small CTAs an SM overlap one another's ends of rows
+    // Few rows: latency counts, a row's loads are spread over four times the threads; more rows than SMs: several
+    // small CTAs an SM overlap one another's ends of rows.  1024 / 256 threads, us, bf16 logits from HBM, 5
+    // alternatives: 65536 wide, 8 rows 12.2 / 16.1, 148 rows 13.9 / 17.5, 149 rows 23.1 / 17.5, 1200 rows 102 / 48;
+    // 32768 wide, 148 rows 11.4 / 11.3, 149 rows 19.4 / 11.4.  Away from these widths the switch is less well placed:
+    // 8192 wide, 8 rows 8.7 / 4.9; 151936 wide, 149 rows 34.5 / 47.7, 300 rows 52 / 56.
     const bool few = rows <= at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
     if (top > 0) {
       if (few) fwd_kernel<T, true, 1024><<<(int)rows, 1024, 0, st>>>(p);

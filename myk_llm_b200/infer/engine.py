@@ -269,8 +269,9 @@ class StaticDecoder:
         return toks, st
 
     def _live_tensors(self) -> list[torch.Tensor]:
-        """Decoder state a round mutates besides the attention caches (whose writes land
-        beyond ``seqlens`` and are harmless to repeat)."""
+        """Decoder state a round mutates besides the attention caches, whose writes are harmless
+        to repeat: they land beyond ``seqlens``, and where they raise the scale of an 8-bit block
+        that holds earlier tokens, the same round finds it raised already."""
         out = [self.seqlens, self.pending, self.history, self.bonus, self.drafts, self.out_tokens, self.out_len,
                self.acc_sum, self.acc_depth]
         if self.logprobs is not None:

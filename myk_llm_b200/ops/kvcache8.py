@@ -13,7 +13,10 @@ scale is the smallest power of two that brings the block's largest magnitude wit
   reads back as NaN until it is written again from its first token on.
 * ``kv8_read`` returns a range of the cache in bf16 (exact: 8-bit values times powers of two).
 * ``flash_attn_with_kvcache8`` is :func:`~myk_llm_b200.ops.attention.flash_attn_with_kvcache`
-  over such a cache: same alignment of queries, windows and empty rows.
+  over such a cache: same alignment of queries, windows and empty rows.  A query that sees a
+  block holding a NaN or an infinity gets NaN, no other does.  Calls of many queries (where it
+  is faster, by a rule on sizes) read the cache's whole capacity back to bf16 for the time of
+  the call and round the weights to 8 bits instead of 11.
 
 As for the bf16 cache, nothing synchronises with the host, tokens past the capacity are
 dropped, the caller advances ``cache_seqlens``, and there is no backward pass.  On CUDA the
